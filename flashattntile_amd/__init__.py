@@ -21,6 +21,7 @@ from .kernels.decode import (DecodeLaunch, paged_decode_attention, paged_decode_
 from .kernels.prefill import paged_prefill_attention, prefill_attention
 from .ops import (PAGED_DECODE_MULTI_OP, PAGED_DECODE_OP, PAGED_DECODE_QUANT_OP, PREFILL_OP, PREFILL_PAGED_OP,
                   paged_decode, paged_decode_multi, paged_decode_quant, prefill_paged, prefill_varlen)
+from .page_ops import compact_pages, copy_pages, fork_sequences, free_sequences
 from .paging import (AppendLaunch, PagedKVCache, allocate, append_tokens, gather_contiguous, gather_paged,
                      validate_cache)
 from .quant import QuantScales, dequantize_cache, kv_bytes_per_token, quantize_cache
@@ -50,6 +51,10 @@ __all__ = [
     "gather_contiguous",
     "gather_paged",
     "validate_cache",
+    "copy_pages",
+    "fork_sequences",
+    "free_sequences",
+    "compact_pages",
     "QuantScales",
     "quantize_cache",
     "dequantize_cache",

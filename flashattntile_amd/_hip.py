@@ -21,7 +21,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libfat_hip.so"
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 # enum fat_dtype
 DT_F16 = 0
@@ -63,6 +63,11 @@ EXPORTED_SYMBOLS = (
     "fat_prefill_paged",
     "fat_quantize_pages",
     "fat_append_kv",
+    "fat_pages_workspace_bytes",
+    "fat_copy_pages",
+    "fat_fork_sequences",
+    "fat_free_sequences",
+    "fat_compact_pages",
     "fat_cache_stats",
     "fat_check_begin",
     "fat_check_wait",
@@ -281,12 +286,112 @@ class CacheStatsArgs(ctypes.Structure):
     ]
 
 
+class Pool(ctypes.Structure):
+    """Mirror of ``fat_pool``."""
+
+    _fields_ = [
+        ("k_cache", _c_vp),
+        ("v_cache", _c_vp),
+        ("quant_k_cache", _c_vp),
+        ("quant_v_cache", _c_vp),
+        ("k_scale", _c_vp),
+        ("v_scale", _c_vp),
+        ("k_stride_page", _c_i64),
+        ("k_stride_slot", _c_i64),
+        ("k_stride_head", _c_i64),
+        ("v_stride_page", _c_i64),
+        ("v_stride_slot", _c_i64),
+        ("v_stride_head", _c_i64),
+        ("qk_stride_page", _c_i64),
+        ("qk_stride_slot", _c_i64),
+        ("qk_stride_head", _c_i64),
+        ("qv_stride_page", _c_i64),
+        ("qv_stride_slot", _c_i64),
+        ("qv_stride_head", _c_i64),
+        ("scale_stride_page", _c_i64),
+        ("scale_stride_head", _c_i64),
+        ("num_pages", _c_i32),
+        ("page_size", _c_i32),
+        ("num_kv_heads", _c_i32),
+        ("head_dim", _c_i32),
+        ("dtype", _c_i32),
+    ]
+
+
+class CopyPagesArgs(ctypes.Structure):
+    """Mirror of ``fat_copy_pages_args``."""
+
+    _fields_ = [
+        ("pool", Pool),
+        ("src", _c_vp),
+        ("dst", _c_vp),
+        ("count", _c_i64),
+    ]
+
+
+class ForkArgs(ctypes.Structure):
+    """Mirror of ``fat_fork_args``."""
+
+    _fields_ = [
+        ("pool", Pool),
+        ("parents", _c_vp),
+        ("children", _c_vp),
+        ("pages", _c_vp),
+        ("page_table", _c_vp),
+        ("seq_lens", _c_vp),
+        ("page_table_stride", _c_i64),
+        ("batch", _c_i32),
+        ("max_pages", _c_i32),
+        ("count", _c_i32),
+    ]
+
+
+class FreeArgs(ctypes.Structure):
+    """Mirror of ``fat_free_args``."""
+
+    _fields_ = [
+        ("seq_lens", _c_vp),
+        ("held", _c_vp),
+        ("page_table", _c_vp),
+        ("rows", _c_vp),
+        ("pages", _c_vp),
+        ("num_free", _c_vp),
+        ("workspace", _c_vp),
+        ("page_table_stride", _c_i64),
+        ("batch", _c_i32),
+        ("max_pages", _c_i32),
+        ("num_pages", _c_i32),
+        ("page_size", _c_i32),
+        ("count", _c_i32),
+    ]
+
+
+class CompactArgs(ctypes.Structure):
+    """Mirror of ``fat_compact_args``."""
+
+    _fields_ = [
+        ("pool", Pool),
+        ("seq_lens", _c_vp),
+        ("held", _c_vp),
+        ("page_table", _c_vp),
+        ("remap", _c_vp),
+        ("num_used", _c_vp),
+        ("workspace", _c_vp),
+        ("page_table_stride", _c_i64),
+        ("batch", _c_i32),
+        ("max_pages", _c_i32),
+    ]
+
+
 # enum fat_check_kind
 CHECK_CACHE = 0
 CHECK_VARLEN = 1
 CHECK_PAGED = 2
 CHECK_APPEND = 3
 CHECK_RANGE = 4
+CHECK_COPY = 5
+CHECK_FORK = 6
+CHECK_FREE = 7
 CHECK_RESULTS = 16
 CHECK_HOST_WORDS = CHECK_RESULTS + 2 * 64
 
@@ -308,6 +413,9 @@ class CheckArgs(ctypes.Structure):
         ("page_size", _c_i32),
         ("values", _c_vp),
         ("count", _c_i64),
+        ("ids", _c_vp * 3),
+        ("scratch", _c_vp),
+        ("num_pages", _c_i32),
     ]
 
 
@@ -366,6 +474,12 @@ def _load() -> None:
         lib.fat_quantize_pages.argtypes = [ctypes.POINTER(QuantizeArgs), _c_vp]
         lib.fat_append_kv.restype = ctypes.c_int
         lib.fat_append_kv.argtypes = [ctypes.POINTER(AppendArgs), _c_vp]
+        lib.fat_pages_workspace_bytes.restype = ctypes.c_size_t
+        lib.fat_pages_workspace_bytes.argtypes = [_c_i32]
+        for name, args in (("fat_copy_pages", CopyPagesArgs), ("fat_fork_sequences", ForkArgs),
+                           ("fat_free_sequences", FreeArgs), ("fat_compact_pages", CompactArgs)):
+            getattr(lib, name).restype = ctypes.c_int
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), _c_vp]
         lib.fat_cache_stats.restype = ctypes.c_int
         lib.fat_cache_stats.argtypes = [ctypes.POINTER(CacheStatsArgs), _c_vp]
         lib.fat_check_begin.restype = ctypes.c_int
@@ -421,12 +535,19 @@ class Check:
         self._pending = False
 
     def begin(self, kind: int, batch: int, stream: int, cu_q: torch.Tensor | None, cu_k: torch.Tensor | None,
-              seq_lens: torch.Tensor | None, page_table: torch.Tensor | None, page_size: int) -> None:
+              seq_lens: torch.Tensor | None, page_table: torch.Tensor | None, page_size: int, ids=(),
+              scratch: torch.Tensor | None = None, num_pages: int = 0) -> None:
         if self._pending:
             torch.cuda.synchronize(self._device)
         a = self._args
         a.kind = kind
         a.batch = batch
+        if ids:
+            a.count = ids[0].numel()
+            for i, t in enumerate(ids):
+                a.ids[i] = t.data_ptr()
+            a.scratch = _ptr(scratch)
+            a.num_pages = num_pages
         a.cu_q = None if cu_q is None else cu_q.data_ptr()
         a.cu_k = None if cu_k is None else cu_k.data_ptr()
         if seq_lens is not None:
@@ -490,13 +611,16 @@ def float_range(values: torch.Tensor) -> tuple[float, float]:
 
 def check_begin(kind: int, stream: int, device: torch.device, cu_q: torch.Tensor | None = None,
                 cu_k: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None,
-                page_table: torch.Tensor | None = None, page_size: int = 0) -> Check:
+                page_table: torch.Tensor | None = None, page_size: int = 0, ids=(),
+                scratch: torch.Tensor | None = None, num_pages: int = 0) -> Check:
     """Begin a check on ``stream``: ``cu_q`` / ``cu_k`` int32 [B + 1],
     ``seq_lens`` int32 [B] (contiguous), ``page_table`` int32 [B, M > 0] with
-    a unit column stride, B > 0, on one ROCm device."""
+    a unit column stride, B > 0, on one ROCm device; ``ids``: the int32 lists
+    (contiguous, of one length) of a check of page operations, ``scratch`` its
+    int32 scratch memory."""
     check = _thread_check(device)
-    batch = seq_lens.shape[0] if seq_lens is not None else cu_q.shape[0] - 1
-    check.begin(kind, batch, stream, cu_q, cu_k, seq_lens, page_table, page_size)
+    batch = seq_lens.shape[0] if seq_lens is not None else cu_q.shape[0] - 1 if cu_q is not None else 0
+    check.begin(kind, batch, stream, cu_q, cu_k, seq_lens, page_table, page_size, ids, scratch, num_pages)
     return check
 
 
@@ -911,3 +1035,73 @@ def append_args(
 def append_with_args(a: AppendArgs, stream: int) -> None:
     """Enqueue ``fat_append_kv`` with a prepared argument block."""
     _check(lib().fat_append_kv(ctypes.byref(a), _c_vp(stream)), "fat_append_kv")
+
+
+def _set_pool(a: Pool, cache, quantized=None, scales=None) -> None:
+    """Fill ``a`` with the pages of ``cache``, its 8-bit copy ``quantized`` (K
+    and V pages, K and V scales) or, for an 8-bit cache, its ``scales``."""
+    k, v = cache.k_cache, cache.v_cache
+    a.k_cache, a.v_cache = _ptr(k), _ptr(v)
+    a.k_stride_page, a.k_stride_slot, a.k_stride_head = k.stride(0), k.stride(1), k.stride(2)
+    a.v_stride_page, a.v_stride_slot, a.v_stride_head = v.stride(0), v.stride(1), v.stride(2)
+    if quantized is not None:
+        qk, qv, *scales = quantized
+        a.quant_k_cache, a.quant_v_cache = _ptr(qk), _ptr(qv)
+        a.qk_stride_page, a.qk_stride_slot, a.qk_stride_head = qk.stride(0), qk.stride(1), qk.stride(2)
+        a.qv_stride_page, a.qv_stride_slot, a.qv_stride_head = qv.stride(0), qv.stride(1), qv.stride(2)
+    if scales is not None:
+        a.k_scale, a.v_scale = _ptr(scales[0]), _ptr(scales[1])
+        a.scale_stride_page, a.scale_stride_head = scales[0].stride(0), scales[0].stride(1)
+    a.num_pages, a.page_size, a.num_kv_heads, a.head_dim = k.shape
+    a.dtype = dtype_code(k.dtype)
+
+
+def _set_table(a, cache) -> None:
+    a.page_table, a.seq_lens = _ptr(cache.page_table), _ptr(cache.seq_lens)
+    a.page_table_stride = cache.page_table.stride(0)
+    a.batch, a.max_pages = cache.page_table.shape
+
+
+def copy_pages(cache, src: torch.Tensor, dst: torch.Tensor, quantized, scales, stream: int) -> None:
+    """Enqueue ``fat_copy_pages`` of already-validated device tensors
+    (``quantized`` and ``scales`` as :func:`_set_pool` takes them)."""
+    a = CopyPagesArgs()
+    _set_pool(a.pool, cache, quantized, scales)
+    a.src, a.dst, a.count = _ptr(src), _ptr(dst), src.numel()
+    _check(lib().fat_copy_pages(ctypes.byref(a), _c_vp(stream)), "fat_copy_pages")
+
+
+def fork_sequences(cache, parents: torch.Tensor, children: torch.Tensor, pages: torch.Tensor, quantized, scales,
+                   stream: int) -> None:
+    """Enqueue ``fat_fork_sequences``."""
+    a = ForkArgs()
+    _set_pool(a.pool, cache, quantized, scales)
+    _set_table(a, cache)
+    a.parents, a.children, a.pages, a.count = _ptr(parents), _ptr(children), _ptr(pages), parents.numel()
+    _check(lib().fat_fork_sequences(ctypes.byref(a), _c_vp(stream)), "fat_fork_sequences")
+
+
+def pages_workspace(num_pages: int, device: torch.device) -> torch.Tensor:
+    """Workspace of one :func:`free_sequences` or :func:`compact_pages`."""
+    return torch.empty(int(lib().fat_pages_workspace_bytes(num_pages)), dtype=torch.uint8, device=device)
+
+
+def free_sequences(cache, rows: torch.Tensor, held: torch.Tensor | None, pages: torch.Tensor, num_free: torch.Tensor,
+                   workspace: torch.Tensor, stream: int) -> None:
+    """Enqueue ``fat_free_sequences``."""
+    a = FreeArgs()
+    _set_table(a, cache)
+    a.held, a.rows, a.pages, a.num_free = _ptr(held), _ptr(rows), _ptr(pages), _ptr(num_free)
+    a.workspace = _ptr(workspace)
+    a.num_pages, a.page_size, a.count = cache.k_cache.shape[0], cache.page_size, rows.numel()
+    _check(lib().fat_free_sequences(ctypes.byref(a), _c_vp(stream)), "fat_free_sequences")
+
+
+def compact_pages(cache, held: torch.Tensor | None, remap: torch.Tensor, num_used: torch.Tensor,
+                  workspace: torch.Tensor, quantized, scales, stream: int) -> None:
+    """Enqueue ``fat_compact_pages``."""
+    a = CompactArgs()
+    _set_pool(a.pool, cache, quantized, scales)
+    _set_table(a, cache)
+    a.held, a.remap, a.num_used, a.workspace = _ptr(held), _ptr(remap), _ptr(num_used), _ptr(workspace)
+    _check(lib().fat_compact_pages(ctypes.byref(a), _c_vp(stream)), "fat_compact_pages")

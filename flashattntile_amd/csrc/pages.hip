@@ -1,0 +1,666 @@
+// pages.hip -- operations on the pages of a paged cache: copying pages, forking
+// sequences, freeing them and compacting the pool.
+//
+// All of it moves bytes and whole numbers, so what bounds it is HBM where pages
+// are copied and launch latency everywhere else.
+//   copy     page dst[i] := page src[i] of every plane (K, V, their 8-bit copy,
+//            the scales)
+//   fork     the parent's table row, and a copy of its partly filled last page
+//   free     U[id] = 1 if a row's used columns name page id; the ids with U = 0,
+//            ascending
+//   compact  n = sum U; the i-th id >= n with U = 1 goes to the i-th id < n with
+//            U = 0.  Sources and destinations are disjoint, so the copies need
+//            no order, and as many ids < n are unused as ids >= n are used.
+#include <algorithm>
+
+#include "fat_common.h"
+
+namespace fat {
+
+// One tensor of a pool: `outer` x `inner` rows of `row` bytes per page, which
+// the host has merged where they lie behind each other.
+struct Plane {
+  uint8_t* base;
+  int64_t page;             // bytes between pages
+  int64_t outer_stride, inner_stride;
+  uint32_t inner;           // rows per outer step
+  uint32_t vpr;             // vectors per row
+  uint32_t vpp;             // vectors per page
+  uint32_t ppw;             // pages per workgroup step (vpp small), or 1
+  uint32_t spp;             // workgroup steps per page (vpp large), or 1
+  int32_t log2v;            // log2 of the vector's bytes
+};
+
+constexpr int kMaxPlanes = 6;
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 8;  // vectors per thread and step: 32 KiB of 16-byte vectors
+constexpr uint32_t kCopyStep = kCopyThreads * kCopyUnroll;
+
+struct Planes {
+  Plane p[kMaxPlanes];
+  int32_t n;
+  int32_t num_pages;
+};
+
+__device__ __forceinline__ int64_t plane_offset(const Plane& pl, uint32_t v) {
+  if (v < pl.vpr) return (int64_t)v << pl.log2v;  // the first row, or a page that is one row
+  const uint32_t r = v / pl.vpr;
+  const uint32_t o = r / pl.inner;
+  return (int64_t)o * pl.outer_stride + (int64_t)(r - o * pl.inner) * pl.inner_stride +
+         ((int64_t)(v - r * pl.vpr) << pl.log2v);
+}
+
+template <typename V>
+__device__ __forceinline__ void copy_vec(const uint8_t* src, uint8_t* dst) {
+  *reinterpret_cast<V*>(dst) = *reinterpret_cast<const V*>(src);
+}
+
+// The pages of one workgroup step of a plane: pair(i, src, dst) gives the ids
+// of pair i < count and whether it is to be copied.
+template <typename V, typename Pair>
+__device__ __forceinline__ void copy_step(const Plane& pl, int64_t step, int64_t count, Pair pair) {
+  if (pl.ppw == 1) {
+    // 32 KiB of one page: its ids are the same for the whole workgroup.
+    const int64_t i = step / pl.spp;
+    const uint32_t v0 = (uint32_t)(step - i * pl.spp) * kCopyStep;
+    int src, dst;
+    if (!pair(i, src, dst)) return;
+    const uint8_t* s = pl.base + (int64_t)src * pl.page;
+    uint8_t* d = pl.base + (int64_t)dst * pl.page;
+    V x[kCopyUnroll];
+    int64_t off[kCopyUnroll];
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u) {
+      const uint32_t v = v0 + u * kCopyThreads + threadIdx.x;
+      off[u] = plane_offset(pl, v);
+      if (v < pl.vpp) x[u] = *reinterpret_cast<const V*>(s + off[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u) {
+      const uint32_t v = v0 + u * kCopyThreads + threadIdx.x;
+      if (v < pl.vpp) *reinterpret_cast<V*>(d + off[u]) = x[u];
+    }
+    return;
+  }
+  // Several small pages.
+  const uint32_t n = (uint32_t)min((int64_t)pl.ppw, count - step * pl.ppw) * pl.vpp;
+  for (uint32_t l = threadIdx.x; l < n; l += kCopyThreads) {
+    const uint32_t k = l / pl.vpp;
+    int src, dst;
+    if (!pair(step * pl.ppw + k, src, dst)) continue;
+    const int64_t off = plane_offset(pl, l - k * pl.vpp);
+    copy_vec<V>(pl.base + (int64_t)src * pl.page + off, pl.base + (int64_t)dst * pl.page + off);
+  }
+}
+
+__device__ __forceinline__ int64_t plane_steps(const Plane& pl, int64_t count) {
+  return pl.ppw == 1 ? count * pl.spp : (count + pl.ppw - 1) / pl.ppw;
+}
+
+template <typename Pair>
+__device__ __forceinline__ void copy_step_any(const Plane& pl, int64_t step, int64_t count, Pair pair) {
+  switch (pl.log2v) {
+    case 4: copy_step<u32x4>(pl, step, count, pair); break;
+    case 3: copy_step<u32x2>(pl, step, count, pair); break;
+    case 2: copy_step<u32>(pl, step, count, pair); break;
+    case 1: copy_step<uint16_t>(pl, step, count, pair); break;
+    default: copy_step<uint8_t>(pl, step, count, pair); break;
+  }
+}
+
+// blockIdx.y: plane; blockIdx.x: steps of it, the grid's width apart.
+__global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(const Planes planes, const int32_t* __restrict__ src,
+                                                                  const int32_t* __restrict__ dst, int64_t count) {
+  const Plane pl = planes.p[blockIdx.y];
+  const int64_t steps = plane_steps(pl, count);
+  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x)
+    copy_step_any(pl, step, count, [&](int64_t i, int& s, int& d) {
+      s = src[i];
+      d = dst[i];
+      return (unsigned)s < (unsigned)planes.num_pages && (unsigned)d < (unsigned)planes.num_pages;
+    });
+}
+
+// ---------------------------------------------------------------------------
+// Fork
+// ---------------------------------------------------------------------------
+struct ForkParams {
+  Planes planes;
+  const int32_t* parents;
+  const int32_t* children;
+  const int32_t* pages;
+  int32_t* pt;
+  int32_t* lens;
+  int64_t pt_sb;
+  int32_t B, max_pages, P;
+};
+
+// blockIdx.y: the fork; blockIdx.z: a plane of its last page, or (the last) its
+// table row; blockIdx.x: steps.  Every workgroup of a fork reads only its
+// parent's row, which no fork of the call writes, and decides alike.
+__global__ __launch_bounds__(kCopyThreads) void fork_kernel(const ForkParams p) {
+  const int i = blockIdx.y;
+  const int parent = p.parents[i], child = p.children[i];
+  if ((unsigned)parent >= (unsigned)p.B || (unsigned)child >= (unsigned)p.B || parent == child) return;
+  const int len = p.lens[parent];
+  if (len < 0 || len > (int64_t)p.max_pages * p.P) return;
+  const int full = len / p.P;
+  const bool tail = len != full * p.P;
+  const int32_t* from = p.pt + (int64_t)parent * p.pt_sb;
+  int src = 0, dst = 0;
+  if (tail) {
+    src = from[full];
+    dst = p.pages[i];
+    if ((unsigned)src >= (unsigned)p.planes.num_pages || (unsigned)dst >= (unsigned)p.planes.num_pages) return;
+  }
+  if ((int)blockIdx.z == p.planes.n) {
+    int32_t* to = p.pt + (int64_t)child * p.pt_sb;
+    const int step = gridDim.x * kCopyThreads;
+    for (int c = blockIdx.x * kCopyThreads + threadIdx.x; c < full; c += step) to[c] = from[c];
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      if (tail) to[full] = dst;
+      p.lens[child] = len;
+    }
+    return;
+  }
+  if (!tail) return;
+  const Plane pl = p.planes.p[blockIdx.z];
+  const int64_t steps = plane_steps(pl, 1);
+  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x)
+    copy_step_any(pl, step, 1, [&](int64_t, int& s, int& d) {
+      s = src;
+      d = dst;
+      return true;
+    });
+}
+
+// ---------------------------------------------------------------------------
+// Which pages are in use, and lists of them
+// ---------------------------------------------------------------------------
+// A byte per page, not a bit: bytes are plain stores that all write the same
+// value (whatever the order, and each XCD's L2 writes back the bytes it has),
+// where bits would be atomics at the level all XCDs share.
+struct UseParams {
+  int32_t* lens;  // (written for freed rows only)
+  int32_t* held;
+  int32_t* pt;    // (written when compacting only)
+  const int32_t* rows;
+  int64_t pt_sb;
+  int32_t B, max_pages, P, num_pages, nrows;
+  uint8_t* used;     // [groups * kUseGroup]
+  int32_t* counts;   // [groups]: used pages of each kUseGroup ids
+  int32_t* list;     // free: the free pages [num_pages]; compact: destinations
+  int32_t* src;      // compact: sources
+  int32_t* rank;     // compact: a moved page's place in src
+  int32_t* remap;    // compact
+  int32_t* total;    // free: free pages; compact: used pages
+};
+
+constexpr int kUseGroup = 4096;  // ids that one workgroup counts and lists
+constexpr int kUseThreads = 256;
+
+__device__ __forceinline__ int used_columns(const UseParams& p, int b) {
+  const int64_t len = max(p.lens[b], 0);
+  int64_t n = (len + p.P - 1) / p.P;
+  if (p.held) n = max(n, (int64_t)p.held[b]);
+  return (int)min(n, (int64_t)p.max_pages);
+}
+
+// Clears the flags and empties the freed rows.
+__global__ __launch_bounds__(kUseThreads) void use_clear_kernel(const UseParams p, int64_t words) {
+  const int64_t step = (int64_t)gridDim.x * kUseThreads;
+  const int64_t t = (int64_t)blockIdx.x * kUseThreads + threadIdx.x;
+  for (int64_t i = t; i < words; i += step) reinterpret_cast<u32x4*>(p.used)[i] = u32x4{0u, 0u, 0u, 0u};
+  for (int64_t i = t; i < p.nrows; i += step) {
+    const int b = p.rows[i];
+    if ((unsigned)b >= (unsigned)p.B) continue;
+    p.lens[b] = 0;
+    if (p.held) p.held[b] = 0;
+  }
+}
+
+// blockIdx.y: rows, the grid's height apart; blockIdx.x: 1024 columns.
+__global__ __launch_bounds__(kUseThreads) void use_mark_kernel(const UseParams p) {
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const int n = used_columns(p, b);
+    const int32_t* row = p.pt + (int64_t)b * p.pt_sb;
+    const int c0 = blockIdx.x * (4 * kUseThreads) + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int c = c0 + u * kUseThreads;
+      if (c < n) {
+        const int id = row[c];
+        if ((unsigned)id < (unsigned)p.num_pages) p.used[id] = 1;
+      }
+    }
+  }
+}
+
+// Sum over the workgroup (all threads get it) and the sum over the threads before.
+__device__ __forceinline__ int use_scan(int x, int& before) {
+  __shared__ int s[kUseThreads / 64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int y = x;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int z = __shfl_up(y, off);
+    y += lane >= off ? z : 0;
+  }
+  __syncthreads();
+  if (lane == 63) s[w] = y;
+  __syncthreads();
+  int total = 0;
+  before = y - x;
+#pragma unroll
+  for (int k = 0; k < kUseThreads / 64; ++k) {
+    before += k < w ? s[k] : 0;
+    total += s[k];
+  }
+  return total;
+}
+
+__global__ __launch_bounds__(kUseThreads) void use_count_kernel(const UseParams p) {
+  const u32x4 f = reinterpret_cast<const u32x4*>(p.used)[(int64_t)blockIdx.x * kUseThreads + threadIdx.x];
+  int before;
+  const int n = use_scan(__popc(f[0]) + __popc(f[1]) + __popc(f[2]) + __popc(f[3]), before);
+  if (threadIdx.x == 0) p.counts[blockIdx.x] = n;
+}
+
+// Writes the lists: a thread has 16 ids.  COMPACT: sources and destinations of
+// the moves and the new ids of the pages that stay, else the free pages.
+template <bool COMPACT>
+__global__ __launch_bounds__(kUseThreads) void use_list_kernel(const UseParams p) {
+  const int groups = gridDim.x;
+  int mine = 0, all = 0, dummy;
+  for (int i = threadIdx.x; i < groups; i += kUseThreads) {
+    const int c = p.counts[i];
+    all += c;
+    mine += i < (int)blockIdx.x ? c : 0;
+  }
+  const int n = use_scan(all, dummy);
+  const int first = use_scan(mine, dummy);
+  u32x4 f = reinterpret_cast<const u32x4*>(p.used)[(int64_t)blockIdx.x * kUseThreads + threadIdx.x];
+  int rank;  // used ids before this thread's
+  use_scan(__popc(f[0]) + __popc(f[1]) + __popc(f[2]) + __popc(f[3]), rank);
+  rank += first;
+  const int id0 = blockIdx.x * kUseGroup + threadIdx.x * 16;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.total = COMPACT ? n : p.num_pages - n;
+  // COMPACT: used ids below n, from whom the moved ones' ranks count.  They are
+  // the used ids of the whole groups below n and those of its own group.
+  int below = 0;
+  if constexpr (COMPACT) {
+    const int gn = n / kUseGroup;
+    int w = 0;
+    for (int i = threadIdx.x; i < min(gn, groups); i += kUseThreads) w += p.counts[i];
+    below = use_scan(w, dummy);
+    if (gn < groups) {
+      const u32x4 h = reinterpret_cast<const u32x4*>(p.used)[(int64_t)gn * kUseThreads + threadIdx.x];
+      const int k0 = gn * kUseGroup + threadIdx.x * 16;
+      int x = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x += k0 + j < n ? (int)((h[j / 4] >> (8 * (j % 4))) & 1) : 0;
+      below += use_scan(x, dummy);
+    }
+  }
+  const int nfree = p.num_pages - n;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int id = id0 + j;
+    const bool used = (f[j / 4] >> (8 * (j % 4))) & 1;
+    if (id < p.num_pages) {
+      if constexpr (COMPACT) {
+        int to = -1;
+        if (used && id < n) to = id;
+        if (!used && id < n) p.list[id - rank] = id;
+        if (used && id >= n) {
+          p.src[rank - below] = id;
+          p.rank[id] = rank - below;
+        } else {
+          p.remap[id] = to;
+        }
+      } else {
+        if (!used) p.list[id - rank] = id;
+        else p.list[nfree + rank] = -1;
+      }
+    }
+    rank += used ? 1 : 0;
+  }
+  if constexpr (COMPACT) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.counts[groups] = n - below;  // moves
+  }
+}
+
+// The moves: blockIdx.y < n planes: copies of that plane; the last: new ids.
+__global__ __launch_bounds__(kCopyThreads) void compact_apply_kernel(const Planes planes, const UseParams p,
+                                                                     int groups) {
+  const int moves = p.counts[groups];
+  if ((int)blockIdx.y < planes.n) {
+    const Plane pl = planes.p[blockIdx.y];
+    const int64_t steps = plane_steps(pl, moves);
+    for (int64_t step = blockIdx.x; step < steps; step += gridDim.x)
+      copy_step_any(pl, step, moves, [&](int64_t i, int& s, int& d) {
+        s = p.src[i];
+        d = p.list[i];
+        return true;
+      });
+    return;
+  }
+  const int n = *p.total;
+  const int64_t stride = (int64_t)gridDim.x * kCopyThreads;
+  for (int64_t i = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x; i < moves; i += stride) p.remap[p.src[i]] = p.list[i];
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    const int cols = used_columns(p, b);
+    int32_t* row = p.pt + (int64_t)b * p.pt_sb;
+    for (int c = threadIdx.x; c < cols; c += kCopyThreads) {
+      const int id = row[c];
+      if (id >= n && id < p.num_pages) row[c] = p.list[p.rank[id]];
+    }
+  }
+}
+
+}  // namespace fat
+
+// ===========================================================================
+// Host side
+// ===========================================================================
+namespace {
+
+int dtype_bytes(int32_t dtype) {
+  switch (dtype) {
+    case FAT_DTYPE_F16:
+    case FAT_DTYPE_BF16: return 2;
+    case FAT_DTYPE_I8:
+    case FAT_DTYPE_FP8E4M3: return 1;
+    case FAT_DTYPE_F32: return 4;
+    default: return 0;
+  }
+}
+
+// A plane of `slots` x `heads` rows of `row` bytes (byte strides).
+fat::Plane make_plane(void* base, int64_t page, int64_t slots, int64_t slot_stride, int64_t heads, int64_t head_stride,
+                      int64_t row) {
+  // The dimension with the smaller stride inside; a dimension of one element
+  // has no stride of its own.
+  if (heads == 1) head_stride = row;
+  if (slots == 1) slot_stride = heads == 1 ? row : head_stride * heads;
+  int64_t outer = slots, os = slot_stride, inner = heads, is = head_stride;
+  if (os < is) {
+    std::swap(outer, inner);
+    std::swap(os, is);
+  }
+  if (is == row) {  // rows of the inner dimension lie behind each other
+    row *= inner;
+    inner = outer;
+    is = os;
+    outer = 1;
+    os = 0;
+    if (is == row) {
+      row *= inner;
+      inner = 1;
+      is = 0;
+    }
+  }
+  int log2v = 4;
+  const uint64_t bits = (uint64_t)(uintptr_t)base | (uint64_t)page | (uint64_t)(outer > 1 ? os : 0) |
+                        (uint64_t)(inner > 1 ? is : 0) | (uint64_t)row;
+  while (log2v > 0 && (bits & ((1u << log2v) - 1))) --log2v;
+  fat::Plane p{};
+  p.base = static_cast<uint8_t*>(base);
+  p.page = page;
+  p.outer_stride = os;
+  p.inner_stride = is;
+  p.inner = (uint32_t)inner;
+  p.vpr = (uint32_t)(row >> log2v);
+  p.vpp = (uint32_t)(outer * inner * (row >> log2v));
+  p.ppw = std::max<uint32_t>(1, fat::kCopyStep / p.vpp);
+  p.spp = (p.vpp + fat::kCopyStep - 1) / fat::kCopyStep;
+  p.log2v = log2v;
+  return p;
+}
+
+int make_planes(const fat_pool& a, fat::Planes* out, const char* who) {
+  if (!a.k_cache || !a.v_cache || !a.quant_k_cache != !a.quant_v_cache || !a.k_scale != !a.v_scale) {
+    fat_host::set_error("%s: k_cache and v_cache are required, the 8-bit copy and the scales come in pairs", who);
+    return FAT_E_INVALID;
+  }
+  if (a.num_pages <= 0 || a.page_size <= 0 || a.num_kv_heads <= 0 || a.head_dim <= 0) {
+    fat_host::set_error("%s: num_pages, page_size, num_kv_heads and head_dim must be positive", who);
+    return FAT_E_INVALID;
+  }
+  const int64_t eb = dtype_bytes(a.dtype);
+  if (!eb) {
+    fat_host::set_error("%s: unknown dtype %d", who, a.dtype);
+    return FAT_E_UNSUPPORTED;
+  }
+  const int64_t P = a.page_size, H = a.num_kv_heads, D = a.head_dim;
+  if (P > (1 << 30) / D / H || P * H * D * eb > (1 << 30)) {
+    fat_host::set_error("%s: pages of more than 1 GiB", who);
+    return FAT_E_UNSUPPORTED;
+  }
+  auto ok = [&](int64_t sp, int64_t ss, int64_t sh) {
+    return (a.num_pages == 1 || sp > 0) && (P == 1 || ss > 0) && (H == 1 || sh > 0);
+  };
+  if (!ok(a.k_stride_page, a.k_stride_slot, a.k_stride_head) || !ok(a.v_stride_page, a.v_stride_slot, a.v_stride_head) ||
+      (a.quant_k_cache && (!ok(a.qk_stride_page, a.qk_stride_slot, a.qk_stride_head) ||
+                           !ok(a.qv_stride_page, a.qv_stride_slot, a.qv_stride_head))) ||
+      (a.k_scale && ((a.num_pages > 1 && a.scale_stride_page <= 0) || (H > 1 && a.scale_stride_head <= 0)))) {
+    fat_host::set_error("%s: the strides of pages, slots, heads and scales must be positive", who);
+    return FAT_E_INVALID;
+  }
+  out->n = 0;
+  out->num_pages = a.num_pages;
+  auto add = [&](void* base, int64_t b, int64_t sp, int64_t ss, int64_t sh) {
+    out->p[out->n++] = make_plane(base, b * sp, P, b * ss, H, b * sh, b * D);
+  };
+  add(a.k_cache, eb, a.k_stride_page, a.k_stride_slot, a.k_stride_head);
+  add(a.v_cache, eb, a.v_stride_page, a.v_stride_slot, a.v_stride_head);
+  if (a.quant_k_cache) {
+    add(a.quant_k_cache, 1, a.qk_stride_page, a.qk_stride_slot, a.qk_stride_head);
+    add(a.quant_v_cache, 1, a.qv_stride_page, a.qv_stride_slot, a.qv_stride_head);
+  }
+  if (a.k_scale) {
+    out->p[out->n++] = make_plane(a.k_scale, 4 * a.scale_stride_page, 1, 0, H, 4 * a.scale_stride_head, 4);
+    out->p[out->n++] = make_plane(a.v_scale, 4 * a.scale_stride_page, 1, 0, H, 4 * a.scale_stride_head, 4);
+  }
+  return FAT_OK;
+}
+
+int64_t host_steps(const fat::Plane& p, int64_t count) {
+  return p.ppw == 1 ? count * p.spp : (count + p.ppw - 1) / p.ppw;
+}
+
+// Workgroups (of 256 threads) that fill the chip: 8 per CU.
+constexpr int64_t kFullGrid = 8 * 256;
+
+unsigned copy_grid(const fat::Planes& pl, int64_t count) {
+  int64_t most = 1;
+  for (int i = 0; i < pl.n; ++i) most = std::max(most, host_steps(pl.p[i], count));
+  return (unsigned)std::min(most, kFullGrid);
+}
+
+int64_t use_groups(int64_t num_pages) { return (num_pages + fat::kUseGroup - 1) / fat::kUseGroup; }
+
+// Workspace: flags, three id lists, counts (one more: the number of moves).
+void use_workspace(fat::UseParams* p, void* ws) {
+  const int64_t groups = use_groups(p->num_pages);
+  uint8_t* at = static_cast<uint8_t*>(ws);
+  p->used = at;
+  at += groups * fat::kUseGroup;
+  auto ints = [&](int64_t n) {
+    int32_t* r = reinterpret_cast<int32_t*>(at);
+    at += 4 * n;
+    return r;
+  };
+  p->src = ints(groups * fat::kUseGroup);
+  p->rank = ints(groups * fat::kUseGroup);
+  p->list = ints(groups * fat::kUseGroup);
+  p->counts = ints(groups + 1);
+}
+
+bool use_args_ok(const void* lens, const void* pt, int64_t pt_sb, int batch, int max_pages, int num_pages, int P,
+                 const void* ws, const char* who) {
+  if (!lens || !pt || !ws) {
+    fat_host::set_error("%s: a required pointer is NULL", who);
+    return false;
+  }
+  if (batch < 0 || max_pages <= 0 || num_pages <= 0 || num_pages > (1 << 30) || P <= 0 || pt_sb < 0 || (batch > 1 && pt_sb < max_pages) ||
+      (uintptr_t)ws % 16) {
+    fat_host::set_error("%s: batch %d, max_pages %d, num_pages %d, page_size %d, page_table_stride %lld or the "
+                        "workspace's alignment invalid", who, batch, max_pages, num_pages, P, (long long)pt_sb);
+    return false;
+  }
+  return true;
+}
+
+// Flags and counts of the pages in use.
+int launch_use(const fat::UseParams& p, hipStream_t stream) {
+  const int64_t groups = use_groups(p.num_pages);
+  const int64_t words = groups * fat::kUseGroup / 16;
+  const int64_t most = std::max<int64_t>(words, p.nrows);
+  const unsigned clear = (unsigned)std::min<int64_t>((most + fat::kUseThreads - 1) / fat::kUseThreads, kFullGrid);
+  hipLaunchKernelGGL(fat::use_clear_kernel, dim3(clear), dim3(fat::kUseThreads), 0, stream, p, words);
+  int rc = fat_host::launch_status("use_clear_kernel");
+  if (rc != FAT_OK) return rc;
+  if (p.B > 0) {
+    const dim3 grid((unsigned)((p.max_pages + 4 * fat::kUseThreads - 1) / (4 * fat::kUseThreads)),
+                    (unsigned)std::min(p.B, 32768));
+    hipLaunchKernelGGL(fat::use_mark_kernel, grid, dim3(fat::kUseThreads), 0, stream, p);
+    if ((rc = fat_host::launch_status("use_mark_kernel")) != FAT_OK) return rc;
+  }
+  hipLaunchKernelGGL(fat::use_count_kernel, dim3((unsigned)groups), dim3(fat::kUseThreads), 0, stream, p);
+  return fat_host::launch_status("use_count_kernel");
+}
+
+}  // namespace
+
+extern "C" size_t fat_pages_workspace_bytes(int32_t num_pages) {
+  if (num_pages <= 0) return 0;
+  const int64_t groups = use_groups(num_pages);
+  return (size_t)(groups * fat::kUseGroup * 13 + 4 * (groups + 1));
+}
+
+extern "C" int fat_copy_pages(const fat_copy_pages_args* a, void* stream_ptr) {
+  fat_host::clear_error();
+  if (!a || (a->count > 0 && (!a->src || !a->dst))) {
+    fat_host::set_error("fat_copy_pages: src and dst are required");
+    return FAT_E_INVALID;
+  }
+  fat::Planes planes{};
+  int rc = make_planes(a->pool, &planes, "fat_copy_pages");
+  if (rc != FAT_OK) return rc;
+  if (a->count < 0 || a->count > 0x7fffffff) {
+    fat_host::set_error("fat_copy_pages: count must be in [0, 2^31), got %lld", (long long)a->count);
+    return FAT_E_INVALID;
+  }
+  if (a->count == 0) return FAT_OK;
+  hipLaunchKernelGGL(fat::copy_pages_kernel, dim3(copy_grid(planes, a->count), planes.n), dim3(fat::kCopyThreads), 0,
+                     static_cast<hipStream_t>(stream_ptr), planes, a->src, a->dst, a->count);
+  return fat_host::launch_status("copy_pages_kernel");
+}
+
+extern "C" int fat_fork_sequences(const fat_fork_args* a, void* stream_ptr) {
+  fat_host::clear_error();
+  if (!a || !a->page_table || !a->seq_lens || (a->count > 0 && (!a->parents || !a->children || !a->pages))) {
+    fat_host::set_error("fat_fork_sequences: parents, children, pages, page_table and seq_lens are required");
+    return FAT_E_INVALID;
+  }
+  fat::ForkParams prm{};
+  int rc = make_planes(a->pool, &prm.planes, "fat_fork_sequences");
+  if (rc != FAT_OK) return rc;
+  if (a->count < 0 || a->batch <= 0 || a->max_pages <= 0 || (a->batch > 1 && a->page_table_stride < a->max_pages)) {
+    fat_host::set_error("fat_fork_sequences: count %d, batch %d, max_pages %d or page_table_stride %lld invalid",
+                        a->count, a->batch, a->max_pages, (long long)a->page_table_stride);
+    return FAT_E_INVALID;
+  }
+  // More forks than rows give some row twice; and a grid is at most 65535 high.
+  if (a->count > a->batch || a->count > 65535) {
+    fat_host::set_error("fat_fork_sequences: at most min(batch, 65535) forks in a call, got %d", a->count);
+    return FAT_E_INVALID;
+  }
+  if (a->count == 0) return FAT_OK;
+  prm.parents = a->parents;
+  prm.children = a->children;
+  prm.pages = a->pages;
+  prm.pt = a->page_table;
+  prm.lens = a->seq_lens;
+  prm.pt_sb = a->page_table_stride;
+  prm.B = a->batch;
+  prm.max_pages = a->max_pages;
+  prm.P = a->pool.page_size;
+  const unsigned table = (unsigned)std::min<int64_t>((a->max_pages + 1023) / 1024, 64);
+  const dim3 grid(std::max(copy_grid(prm.planes, 1), table), (unsigned)a->count, prm.planes.n + 1);
+  hipLaunchKernelGGL(fat::fork_kernel, grid, dim3(fat::kCopyThreads), 0, static_cast<hipStream_t>(stream_ptr), prm);
+  return fat_host::launch_status("fork_kernel");
+}
+
+extern "C" int fat_free_sequences(const fat_free_args* a, void* stream_ptr) {
+  fat_host::clear_error();
+  if (!a || !a->pages || !a->num_free || (a->count > 0 && !a->rows)) {
+    fat_host::set_error("fat_free_sequences: rows, pages and num_free are required");
+    return FAT_E_INVALID;
+  }
+  if (!use_args_ok(a->seq_lens, a->page_table, a->page_table_stride, a->batch, a->max_pages, a->num_pages,
+                   a->page_size, a->workspace, "fat_free_sequences"))
+    return FAT_E_INVALID;
+  if (a->count < 0) {
+    fat_host::set_error("fat_free_sequences: count must be >= 0, got %d", a->count);
+    return FAT_E_INVALID;
+  }
+  fat::UseParams prm{};
+  prm.lens = a->seq_lens;
+  prm.held = a->held;
+  prm.pt = const_cast<int32_t*>(a->page_table);
+  prm.rows = a->rows;
+  prm.pt_sb = a->page_table_stride;
+  prm.B = a->batch;
+  prm.max_pages = a->max_pages;
+  prm.P = a->page_size;
+  prm.num_pages = a->num_pages;
+  prm.nrows = a->count;
+  use_workspace(&prm, a->workspace);
+  prm.list = a->pages;
+  prm.total = a->num_free;
+  hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+  const int rc = launch_use(prm, stream);
+  if (rc != FAT_OK) return rc;
+  hipLaunchKernelGGL((fat::use_list_kernel<false>), dim3((unsigned)use_groups(a->num_pages)), dim3(fat::kUseThreads), 0,
+                     stream, prm);
+  return fat_host::launch_status("use_list_kernel");
+}
+
+extern "C" int fat_compact_pages(const fat_compact_args* a, void* stream_ptr) {
+  fat_host::clear_error();
+  if (!a || !a->remap || !a->num_used) {
+    fat_host::set_error("fat_compact_pages: remap and num_used are required");
+    return FAT_E_INVALID;
+  }
+  fat::Planes planes{};
+  int rc = make_planes(a->pool, &planes, "fat_compact_pages");
+  if (rc != FAT_OK) return rc;
+  if (!use_args_ok(a->seq_lens, a->page_table, a->page_table_stride, a->batch, a->max_pages, a->pool.num_pages,
+                   a->pool.page_size, a->workspace, "fat_compact_pages"))
+    return FAT_E_INVALID;
+  fat::UseParams prm{};
+  prm.lens = const_cast<int32_t*>(a->seq_lens);
+  prm.held = const_cast<int32_t*>(a->held);
+  prm.pt = a->page_table;
+  prm.pt_sb = a->page_table_stride;
+  prm.B = a->batch;
+  prm.max_pages = a->max_pages;
+  prm.P = a->pool.page_size;
+  prm.num_pages = a->pool.num_pages;
+  use_workspace(&prm, a->workspace);
+  prm.remap = a->remap;
+  prm.total = a->num_used;
+  hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+  if ((rc = launch_use(prm, stream)) != FAT_OK) return rc;
+  const int groups = (int)use_groups(prm.num_pages);
+  hipLaunchKernelGGL((fat::use_list_kernel<true>), dim3((unsigned)groups), dim3(fat::kUseThreads), 0, stream, prm);
+  if ((rc = fat_host::launch_status("use_list_kernel")) != FAT_OK) return rc;
+  // At most half of the pages move; the number is known on the device only.
+  const unsigned wide = std::max(copy_grid(planes, prm.num_pages / 2 + 1),
+                                 (unsigned)std::min<int64_t>(std::max(prm.B, 1), kFullGrid));
+  hipLaunchKernelGGL(fat::compact_apply_kernel, dim3(wide, planes.n + 1), dim3(fat::kCopyThreads), 0, stream, planes,
+                     prm, groups);
+  return fat_host::launch_status("compact_apply_kernel");
+}

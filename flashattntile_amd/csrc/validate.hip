@@ -118,6 +118,9 @@ struct CheckParams {
   int32_t B, max_pages, P;
   const float* values;
   int64_t count;
+  const int32_t* ids[3];
+  int32_t* scratch;
+  int32_t num_pages;
 };
 
 struct RMin { template <typename T> static __device__ __forceinline__ T f(T a, T b) { return a < b ? a : b; } };
@@ -146,9 +149,9 @@ __device__ __forceinline__ long long check_reduce(long long x) {
 // so no cache is written back and the host needs no synchronisation.
 template <int KIND>
 __global__ __launch_bounds__(kCheckThreads) void check_kernel(const CheckParams p) {
-  constexpr bool LENS = KIND == FAT_CHECK_CACHE || KIND == FAT_CHECK_PAGED || KIND == FAT_CHECK_APPEND;
+  constexpr bool TABLE = KIND == FAT_CHECK_CACHE || KIND == FAT_CHECK_PAGED || KIND == FAT_CHECK_FREE;
+  constexpr bool LENS = TABLE || KIND == FAT_CHECK_APPEND;
   constexpr bool CU = KIND == FAT_CHECK_VARLEN || KIND == FAT_CHECK_PAGED;
-  constexpr bool TABLE = KIND == FAT_CHECK_CACHE || KIND == FAT_CHECK_PAGED;
   const int tid = threadIdx.x;
   auto put = [&](int word, long long v) {
     __hip_atomic_store(p.host + word, (int64_t)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
@@ -228,6 +231,11 @@ __global__ __launch_bounds__(kCheckThreads) void check_kernel(const CheckParams 
       mk = check_reduce<RMax>(mk);
       keyless = check_reduce<RMin>(keyless);
     }
+    if constexpr (KIND == FAT_CHECK_FREE) {
+      for (int64_t i = tid; i < p.count; i += kCheckThreads) flags |= (unsigned)p.ids[0][i] >= (unsigned)p.B ? 1 : 0;
+      flags = check_reduce<ROr>(flags);
+      if (tid == 0) put(7, flags);
+    }
     if (tid == 0) {
       put(0, mn);
       put(1, mx);
@@ -258,12 +266,99 @@ __global__ __launch_bounds__(kCheckThreads) void check_kernel(const CheckParams 
   }
 }
 
+// COPY and FORK: ranges, and ids that are given twice or on both sides.  An id
+// d of list b is "owned" by the last writer of own[d], and own needs no
+// clearing: own[x] names an element k only if 0 <= k < count and b[k] == x, so
+// what memory held before never counts.  One workgroup (its threads have to see
+// each other's stores); 8192 pairs take as long as the launch itself.
+constexpr int kListThreads = 1024;
+
+__device__ __forceinline__ int own_load(const int32_t* own, int x) {
+  return __hip_atomic_load(own + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void own_store(int32_t* own, int x, int k) {
+  __hip_atomic_store(own + x, k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whether x is an element of list b[0 .. n - 1], by the owners.
+__device__ __forceinline__ bool owned(const int32_t* own, const int32_t* b, int64_t n, int x) {
+  const int k = own_load(own, x);
+  return (unsigned)k < (unsigned)n && b[k] == x;
+}
+
+template <int KIND>
+__global__ __launch_bounds__(kListThreads) void check_lists_kernel(const CheckParams p) {
+  constexpr bool FORK = KIND == FAT_CHECK_FORK;
+  const int tid = threadIdx.x;
+  const int n = (int)p.count;
+  const int32_t* a = p.ids[0];
+  const int32_t* b = p.ids[1];
+  const int32_t* pages = p.ids[2];
+  const unsigned limit = FORK ? p.B : p.num_pages;
+  int32_t* own = p.scratch;                    // [limit]
+  int32_t* own_pages = p.scratch + p.B;        // FORK: [num_pages]
+  int flags = 0;
+  // FORK: whether fork i's parent ends inside a page (its pages[i] is used).
+  auto tail = [&](int i, int& len) {
+    const int parent = a[i];
+    len = (unsigned)parent < limit ? p.lens[parent] : 0;
+    return len > 0 && len <= (int64_t)p.max_pages * p.P && len % p.P != 0;
+  };
+#pragma unroll 4
+  for (int i = tid; i < n; i += kListThreads) {
+    const int x = a[i], y = b[i];
+    flags |= (unsigned)x >= limit ? 1 : 0;
+    if ((unsigned)y >= limit) flags |= 2;
+    else own_store(own, y, i);
+    if constexpr (FORK) {
+      int len;
+      if ((unsigned)y < limit && p.lens[y] != 0) flags |= 16;
+      if (tail(i, len)) {
+        if ((unsigned)p.pt[x * p.pt_sb + len / p.P] >= (unsigned)p.num_pages) flags |= 64;
+        if ((unsigned)pages[i] >= (unsigned)p.num_pages) flags |= 128;
+        else own_store(own_pages, pages[i], i);
+      }
+      if (len < 0 || len > (int64_t)p.max_pages * p.P) flags |= 32;
+    }
+  }
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's stores are complete
+  __syncthreads();
+#pragma unroll 4
+  for (int i = tid; i < n; i += kListThreads) {
+    const int x = a[i], y = b[i];
+    if ((unsigned)y < limit && own_load(own, y) != i) flags |= 4;
+    if ((unsigned)x < limit && owned(own, b, n, x)) flags |= 8;
+    if constexpr (FORK) {
+      int len;
+      if (tail(i, len) && (unsigned)pages[i] < (unsigned)p.num_pages && own_load(own_pages, pages[i]) != i)
+        flags |= 256;
+    }
+  }
+  __shared__ int s_flags;
+  if (tid == 0) s_flags = 0;
+  __syncthreads();
+  if (flags) atomicOr(&s_flags, flags);
+  __syncthreads();
+  if (tid == 0) {
+    auto put = [&](int word, long long v) {
+      __hip_atomic_store(p.host + word, (int64_t)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    };
+    put(7, s_flags);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the result is complete
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    put(FAT_CHECK_RESULTS + 1, p.ticket);
+  }
+}
+
 }  // namespace fat
 
 namespace {
 
 int check_groups(const fat_check_args* a) {
-  if (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_APPEND) return 1;
+  if (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_APPEND || a->kind == FAT_CHECK_COPY ||
+      a->kind == FAT_CHECK_FORK)
+    return 1;
   const int64_t entries = a->kind == FAT_CHECK_RANGE ? a->count : (int64_t)a->batch * a->max_pages;
   const int64_t n = (entries + fat::kCheckEntries - 1) / fat::kCheckEntries;
   return (int)std::min<int64_t>(std::max<int64_t>(n, 1), FAT_CHECK_MAX_GROUPS);
@@ -272,14 +367,18 @@ int check_groups(const fat_check_args* a) {
 bool check_args_ok(const fat_check_args* a, const char* who) {
   const bool cu = a && (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_PAGED);
   const bool range = a && a->kind == FAT_CHECK_RANGE;
-  const bool lens = a && a->kind != FAT_CHECK_VARLEN && !range;
-  if (!a || !a->host || (cu && !a->cu_q) || (a->kind == FAT_CHECK_VARLEN && !a->cu_k) || (lens && !a->seq_lens) ||
+  const bool copy = a && a->kind == FAT_CHECK_COPY, fork = a && a->kind == FAT_CHECK_FORK;
+  const bool lens = a && a->kind != FAT_CHECK_VARLEN && !range && !copy;
+  const bool ids = copy || fork || (a && a->kind == FAT_CHECK_FREE && a->count > 0);
+  if (!a || !a->host || (ids && !a->ids[0]) || ((copy || fork) && (!a->ids[1] || !a->scratch)) ||
+      (fork && !a->ids[2]) || (cu && !a->cu_q) || (a->kind == FAT_CHECK_VARLEN && !a->cu_k) || (lens && !a->seq_lens) ||
       (lens && !a->page_table) || (range && !a->values)) {
     fat_host::set_error("%s: a required pointer is NULL", who);
     return false;
   }
-  if (a->kind < FAT_CHECK_CACHE || a->kind > FAT_CHECK_RANGE || (!range && a->batch <= 0) ||
-      a->ticket <= 0 || (range && a->count <= 0) ||
+  if (a->kind < FAT_CHECK_CACHE || a->kind > FAT_CHECK_FREE || (!range && !copy && a->batch <= 0) ||
+      a->ticket <= 0 || (range && a->count <= 0) || (a->kind == FAT_CHECK_FREE && a->count < 0) ||
+      ((copy || fork) && (a->count <= 0 || a->count > INT_MAX || a->num_pages <= 0)) ||
       (lens && (a->max_pages <= 0 || a->page_size <= 0 || a->page_table_stride < 0)) ||
       (a->kind == FAT_CHECK_CACHE && a->page_table_stride < a->max_pages)) {
     fat_host::set_error("%s: kind %d, batch %d, ticket %lld, max_pages %d, page_size %d or page_table_stride %lld "
@@ -305,13 +404,21 @@ extern "C" int fat_check_begin(const fat_check_args* a, void* stream_ptr) {
     return FAT_E_LAUNCH;
   }
   const fat::CheckParams prm{a->cu_q, a->cu_k, a->seq_lens, a->page_table, a->page_table_stride, a->host,
-                             a->ticket, a->batch, a->max_pages, a->page_size, a->values, a->count};
+                             a->ticket, a->batch, a->max_pages, a->page_size, a->values, a->count,
+                             {a->ids[0], a->ids[1], a->ids[2]}, a->scratch, a->num_pages};
   const dim3 grid((unsigned)check_groups(a)), block(fat::kCheckThreads);
   switch (a->kind) {
     case FAT_CHECK_CACHE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_CACHE>), grid, block, 0, stream, prm); break;
     case FAT_CHECK_VARLEN: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_VARLEN>), grid, block, 0, stream, prm); break;
     case FAT_CHECK_PAGED: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_PAGED>), grid, block, 0, stream, prm); break;
     case FAT_CHECK_RANGE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_RANGE>), grid, block, 0, stream, prm); break;
+    case FAT_CHECK_FREE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_FREE>), grid, block, 0, stream, prm); break;
+    case FAT_CHECK_COPY:
+      hipLaunchKernelGGL((fat::check_lists_kernel<FAT_CHECK_COPY>), grid, dim3(fat::kListThreads), 0, stream, prm);
+      break;
+    case FAT_CHECK_FORK:
+      hipLaunchKernelGGL((fat::check_lists_kernel<FAT_CHECK_FORK>), grid, dim3(fat::kListThreads), 0, stream, prm);
+      break;
     default: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_APPEND>), grid, block, 0, stream, prm); break;
   }
   return fat_host::launch_status("check_kernel");

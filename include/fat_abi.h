@@ -46,7 +46,9 @@
 extern "C" {
 #endif
 
-/* 17: fat_decode_args.workspace_bytes; fat_stream_capture_id.
+/* 18: operations on pages (fat_copy_pages, fat_fork_sequences,
+ *     fat_free_sequences, fat_compact_pages) and FAT_CHECK_COPY, _FORK, _FREE.
+ * 17: fat_decode_args.workspace_bytes; fat_stream_capture_id.
  * 16: fat_prefill_paged_args.v_workspace, .total_k and fat_prefill_paged_v_bytes:
  *     chunks of long contexts on the wide kernel, K read through the pages.
  * 15: fat_decode_args.balanced; fat_check_begin / fat_check_wait (one launch and one host poll per
@@ -68,7 +70,7 @@ extern "C" {
  * 8: fp32 decode, any page size and head_dim 32/256 through the generic
  *    decode kernel (FAT_KERNEL_DECODE_GENERIC); the paged prefill `rows`
  *    field replaces the library's environment overrides. */
-#define FAT_ABI_VERSION 17
+#define FAT_ABI_VERSION 18
 
 /* Element types understood by the kernels. */
 enum fat_dtype {
@@ -508,6 +510,118 @@ int fat_quantize_pages(const fat_quantize_args* args, void* stream);
 int fat_append_kv(const fat_append_args* args, void* stream);
 
 /*
+ * Operations on the pages of a cache (no reference counterpart: its engine
+ * neither shares pages nor moves them).
+ *
+ * A pool: K and V pages [num_pages, page_size, num_kv_heads, head_dim] of any
+ * fat_dtype and any strides (in elements, head_dim contiguous), an optional
+ * 8-bit copy of them (quant_k_cache and quant_v_cache, both or neither) and
+ * optional fp32 scales [num_pages, num_kv_heads] (of the copy, or of an 8-bit
+ * cache).  Whatever is given moves together.  All bytes of a page are copied,
+ * the slots behind a sequence's end among them (a page's scales depend on
+ * every slot of it).
+ */
+typedef struct fat_pool {
+  void* k_cache;
+  void* v_cache;
+  void* quant_k_cache;
+  void* quant_v_cache;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_stride_page, k_stride_slot, k_stride_head;
+  int64_t v_stride_page, v_stride_slot, v_stride_head;
+  int64_t qk_stride_page, qk_stride_slot, qk_stride_head;
+  int64_t qv_stride_page, qv_stride_slot, qv_stride_head;
+  int64_t scale_stride_page, scale_stride_head; /* shared by k/v_scale */
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t dtype; /* any fat_dtype */
+} fat_pool;
+
+/* Page dst[i] := page src[i] for i < count.  No dst may be given twice or be a
+ * src of the call too; a pair with an id outside [0, num_pages) is skipped. */
+typedef struct fat_copy_pages_args {
+  fat_pool pool;
+  const int32_t* src;
+  const int32_t* dst;
+  int64_t count;
+} fat_copy_pages_args;
+
+/* Row children[i] of the table becomes a fork of row parents[i] (i < count): n
+ * = seq_lens[parent] tokens, the same pages, but, where n is no multiple of
+ * page_size, a copy of the last one in page pages[i]; seq_lens[child] = n.
+ * Table columns behind ceil(n / page_size) stay as they are.  No child may be
+ * given twice or be a parent of the call too, and no sequence may use
+ * pages[i].  A fork with a row, length or page that is out of range is
+ * skipped whole. */
+typedef struct fat_fork_args {
+  fat_pool pool;
+  const int32_t* parents;
+  const int32_t* children;
+  const int32_t* pages;
+  int32_t* page_table; /* [batch, max_pages], row stride page_table_stride */
+  int32_t* seq_lens;   /* [batch] */
+  int64_t page_table_stride;
+  int32_t batch;
+  int32_t max_pages;
+  int32_t count;
+} fat_fork_args;
+
+/* seq_lens[rows[i]] = 0 (and held[rows[i]] = 0) for i < count, then the pages
+ * that no row uses, ascending, in pages[0 .. n - 1], -1 in pages[n ..
+ * num_pages - 1], and n in *num_free.  Row b uses the pages in its first
+ * max(ceil(seq_lens[b] / page_size), held[b]) columns; held is optional (pages
+ * that an engine has given a row ahead of its tokens).  Rows out of range and
+ * table entries outside [0, num_pages) are skipped.  workspace: at least
+ * fat_pages_workspace_bytes(num_pages) bytes, 16-byte aligned. */
+typedef struct fat_free_args {
+  int32_t* seq_lens;         /* [batch] */
+  int32_t* held;             /* [batch] or NULL */
+  const int32_t* page_table; /* [batch, max_pages], row stride page_table_stride */
+  const int32_t* rows;       /* [count] */
+  int32_t* pages;            /* [num_pages] */
+  int32_t* num_free;         /* [1] */
+  void* workspace;
+  int64_t page_table_stride;
+  int32_t batch;
+  int32_t max_pages;
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t count;
+} fat_free_args;
+
+/* Moves the n pages that the table's rows use (as fat_free_args says) to the
+ * pool's front: the i-th used page with an id >= n goes to the i-th unused id
+ * < n, the others stay, and the used columns of the table are renumbered.
+ * remap[id] = a page's new id, -1 for unused pages; *num_used = n.  Pages from
+ * n on keep their bytes. */
+typedef struct fat_compact_args {
+  fat_pool pool;
+  const int32_t* seq_lens; /* [batch] */
+  const int32_t* held;     /* [batch] or NULL */
+  int32_t* page_table;     /* [batch, max_pages], row stride page_table_stride */
+  int32_t* remap;          /* [num_pages] */
+  int32_t* num_used;       /* [1] */
+  void* workspace;
+  int64_t page_table_stride;
+  int32_t batch;
+  int32_t max_pages;
+} fat_compact_args;
+
+/* Bytes of workspace of fat_free_sequences and fat_compact_pages.  Two launches
+ * that may run at the same time need one each. */
+size_t fat_pages_workspace_bytes(int32_t num_pages);
+
+/* Enqueue them on `stream`.  None allocates, synchronises or needs memory
+ * cleared before it. */
+int fat_copy_pages(const fat_copy_pages_args* args, void* stream);
+int fat_fork_sequences(const fat_fork_args* args, void* stream);
+int fat_free_sequences(const fat_free_args* args, void* stream);
+int fat_compact_pages(const fat_compact_args* args, void* stream);
+
+/*
  * The numbers a paged-cache validation checks, in one launch.
  *   seq_lens   int32 [batch]
  *   page_table int32 [batch, max_pages] (row stride page_table_stride >= max_pages)
@@ -546,6 +660,10 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *                          (flashattn_tile/paging.py:191-205)
  *        FAT_CHECK_RANGE   min and max of values[0 .. count - 1]
  *                          (flashattn_tile/quant.py:128-142, the scale range)
+ *        FAT_CHECK_COPY    src = ids[0] and dst = ids[1], `count` pages each
+ *        FAT_CHECK_FORK    parents, children and pages = ids[0 .. 2], `count`
+ *                          each, with seq_lens and the page table
+ *        FAT_CHECK_FREE    FAT_CHECK_CACHE, and rows = ids[0], `count` of them
  *   host   int64 [FAT_CHECK_HOST_WORDS]: page-locked host memory that the
  *          device can write, zero before its first use and used by one call
  *          at a time
@@ -564,14 +682,26 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *          INT32_MIN when no column is used), or of the entries
  *          [b, clamp(floor(seq_lens[b] / page_size), 0, max_pages - 1)] (APPEND);
  *          the bits of the fp32 min and max, NaN if a value is (RANGE)
- * Entries that a kind doesn't name are undefined.
+ *   7      COPY: 1 a src, 2 a dst out of [0, num_pages), 4 a dst given twice, 8
+ *          a dst that is a src too; FREE: 1 a row out of [0, batch); FORK: 1 a
+ *          parent, 2 a child out of [0, batch), 4 a child given twice, 8 a
+ *          child that is a parent too, 16 a child that holds tokens, 32 a
+ *          parent longer than the table or negative, and of parents that end
+ *          inside a page: 64 that page, 128 pages[i] out of [0, num_pages),
+ *          256 pages[i] given twice
+ * Entries that a kind doesn't name are undefined.  `scratch` (COPY: int32
+ * [num_pages], FORK: int32 [num_pages + batch], device memory) need not be
+ * cleared and holds nothing afterwards.
  */
 enum fat_check_kind {
   FAT_CHECK_CACHE = 0,
   FAT_CHECK_VARLEN = 1,
   FAT_CHECK_PAGED = 2,
   FAT_CHECK_APPEND = 3,
-  FAT_CHECK_RANGE = 4
+  FAT_CHECK_RANGE = 4,
+  FAT_CHECK_COPY = 5,
+  FAT_CHECK_FORK = 6,
+  FAT_CHECK_FREE = 7
 };
 #define FAT_CHECK_RESULTS 16
 #define FAT_CHECK_MAX_GROUPS 64
@@ -590,6 +720,9 @@ typedef struct fat_check_args {
   int32_t page_size;
   const float* values; /* [count], RANGE only */
   int64_t count;
+  const int32_t* ids[3]; /* [count] each: COPY, FORK and FREE only */
+  int32_t* scratch;
+  int32_t num_pages; /* COPY and FORK only */
 } fat_check_args;
 
 /* Enqueue the check on `stream`.  FAT_E_LAUNCH while the stream is capturing
