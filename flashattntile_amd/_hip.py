@@ -21,7 +21,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libfat_hip.so"
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 # enum fat_dtype
 DT_F16 = 0
@@ -55,6 +55,8 @@ EXPORTED_SYMBOLS = (
     "fat_paged_decode_balanced_workspace_bytes",
     "fat_paged_decode",
     "fat_paged_decode_noalloc",
+    "fat_paged_decode_shared_workspace_bytes",
+    "fat_paged_decode_shared",
     "fat_prefill_workspace_bytes",
     "fat_prefill_varlen_workspace_bytes",
     "fat_prefill_varlen",
@@ -286,6 +288,57 @@ class CacheStatsArgs(ctypes.Structure):
     ]
 
 
+class SharedArgs(ctypes.Structure):
+    """Mirror of ``fat_shared_args``."""
+
+    _fields_ = [
+        ("q", _c_vp),
+        ("k_cache", _c_vp),
+        ("v_cache", _c_vp),
+        ("k_scale", _c_vp),
+        ("v_scale", _c_vp),
+        ("page_table", _c_vp),
+        ("seq_lens", _c_vp),
+        ("cu_groups", _c_vp),
+        ("prefix_lens", _c_vp),
+        ("out", _c_vp),
+        ("workspace", _c_vp),
+        ("workspace_bytes", _c_i64),
+        ("q_stride_b", _c_i64),
+        ("q_stride_t", _c_i64),
+        ("q_stride_h", _c_i64),
+        ("k_stride_page", _c_i64),
+        ("k_stride_slot", _c_i64),
+        ("k_stride_head", _c_i64),
+        ("v_stride_page", _c_i64),
+        ("v_stride_slot", _c_i64),
+        ("v_stride_head", _c_i64),
+        ("scale_stride_page", _c_i64),
+        ("scale_stride_head", _c_i64),
+        ("page_table_stride", _c_i64),
+        ("out_stride_b", _c_i64),
+        ("out_stride_t", _c_i64),
+        ("out_stride_h", _c_i64),
+        ("batch", _c_i32),
+        ("groups", _c_i32),
+        ("max_group", _c_i32),
+        ("num_heads", _c_i32),
+        ("num_kv_heads", _c_i32),
+        ("head_dim", _c_i32),
+        ("page_size", _c_i32),
+        ("num_pages", _c_i32),
+        ("max_pages", _c_i32),
+        ("q_len", _c_i32),
+        ("q_dtype", _c_i32),
+        ("kv_dtype", _c_i32),
+        ("prefix_split", _c_i32),
+        ("prefix_chunk", _c_i32),
+        ("split", _c_i32),
+        ("chunk", _c_i32),
+        ("softmax_scale", ctypes.c_float),
+    ]
+
+
 class Pool(ctypes.Structure):
     """Mirror of ``fat_pool``."""
 
@@ -392,6 +445,7 @@ CHECK_RANGE = 4
 CHECK_COPY = 5
 CHECK_FORK = 6
 CHECK_FREE = 7
+CHECK_SHARED = 8
 CHECK_RESULTS = 16
 CHECK_HOST_WORDS = CHECK_RESULTS + 2 * 64
 
@@ -416,6 +470,7 @@ class CheckArgs(ctypes.Structure):
         ("ids", _c_vp * 3),
         ("scratch", _c_vp),
         ("num_pages", _c_i32),
+        ("tokens", _c_i32),
     ]
 
 
@@ -474,6 +529,10 @@ def _load() -> None:
         lib.fat_quantize_pages.argtypes = [ctypes.POINTER(QuantizeArgs), _c_vp]
         lib.fat_append_kv.restype = ctypes.c_int
         lib.fat_append_kv.argtypes = [ctypes.POINTER(AppendArgs), _c_vp]
+        lib.fat_paged_decode_shared_workspace_bytes.restype = ctypes.c_size_t
+        lib.fat_paged_decode_shared_workspace_bytes.argtypes = [_c_i32, _c_i32, _c_i32, _c_i32]
+        lib.fat_paged_decode_shared.restype = ctypes.c_int
+        lib.fat_paged_decode_shared.argtypes = [ctypes.POINTER(SharedArgs), _c_vp]
         lib.fat_pages_workspace_bytes.restype = ctypes.c_size_t
         lib.fat_pages_workspace_bytes.argtypes = [_c_i32]
         for name, args in (("fat_copy_pages", CopyPagesArgs), ("fat_fork_sequences", ForkArgs),
@@ -536,7 +595,7 @@ class Check:
 
     def begin(self, kind: int, batch: int, stream: int, cu_q: torch.Tensor | None, cu_k: torch.Tensor | None,
               seq_lens: torch.Tensor | None, page_table: torch.Tensor | None, page_size: int, ids=(),
-              scratch: torch.Tensor | None = None, num_pages: int = 0) -> None:
+              scratch: torch.Tensor | None = None, num_pages: int = 0, tokens: int = 1) -> None:
         if self._pending:
             torch.cuda.synchronize(self._device)
         a = self._args
@@ -548,6 +607,7 @@ class Check:
                 a.ids[i] = t.data_ptr()
             a.scratch = _ptr(scratch)
             a.num_pages = num_pages
+            a.tokens = tokens
         a.cu_q = None if cu_q is None else cu_q.data_ptr()
         a.cu_k = None if cu_k is None else cu_k.data_ptr()
         if seq_lens is not None:
@@ -612,15 +672,17 @@ def float_range(values: torch.Tensor) -> tuple[float, float]:
 def check_begin(kind: int, stream: int, device: torch.device, cu_q: torch.Tensor | None = None,
                 cu_k: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None,
                 page_table: torch.Tensor | None = None, page_size: int = 0, ids=(),
-                scratch: torch.Tensor | None = None, num_pages: int = 0) -> Check:
+                scratch: torch.Tensor | None = None, num_pages: int = 0, tokens: int = 1) -> Check:
     """Begin a check on ``stream``: ``cu_q`` / ``cu_k`` int32 [B + 1],
     ``seq_lens`` int32 [B] (contiguous), ``page_table`` int32 [B, M > 0] with
     a unit column stride, B > 0, on one ROCm device; ``ids``: the int32 lists
     (contiguous, of one length) of a check of page operations, ``scratch`` its
-    int32 scratch memory."""
+    int32 scratch memory; of a shared-prefix decode the prefixes, with its
+    ``tokens`` per sequence."""
     check = _thread_check(device)
     batch = seq_lens.shape[0] if seq_lens is not None else cu_q.shape[0] - 1 if cu_q is not None else 0
-    check.begin(kind, batch, stream, cu_q, cu_k, seq_lens, page_table, page_size, ids, scratch, num_pages)
+    check.begin(kind, batch, stream, cu_q, cu_k, seq_lens, page_table, page_size, ids, scratch, num_pages,
+                tokens)
     return check
 
 
@@ -796,6 +858,44 @@ def set_workspace(a: DecodeArgs, workspace: torch.Tensor | None) -> None:
 def decode_with_args(a: DecodeArgs, stream: int) -> None:
     """Enqueue ``fat_paged_decode`` with a prepared argument block."""
     _check(lib().fat_paged_decode(ctypes.byref(a), _c_vp(stream)), "fat_paged_decode")
+
+
+def shared_args(q: torch.Tensor, cache, cu_groups: torch.Tensor, prefix_lens: torch.Tensor, out: torch.Tensor,
+                softmax_scale: float, k_scale: torch.Tensor | None = None,
+                v_scale: torch.Tensor | None = None) -> SharedArgs:
+    """The ``fat_shared_args`` block of a launch but for its splits and
+    workspace (:func:`shared_with_args`).  It holds the tensors' addresses."""
+    a = SharedArgs()
+    k, v, table = cache.k_cache, cache.v_cache, cache.page_table
+    a.q, a.k_cache, a.v_cache, a.k_scale, a.v_scale = _ptr(q), _ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale)
+    a.page_table, a.seq_lens, a.out = _ptr(table), _ptr(cache.seq_lens), _ptr(out)
+    a.cu_groups, a.prefix_lens = _ptr(cu_groups), _ptr(prefix_lens)
+    if q.dim() == 4:
+        a.q_stride_t, a.out_stride_t, a.q_len = q.stride(1), out.stride(1), q.shape[1]
+    a.q_stride_b, a.q_stride_h = q.stride(0), q.stride(-2)
+    a.out_stride_b, a.out_stride_h = out.stride(0), out.stride(-2)
+    a.k_stride_page, a.k_stride_slot, a.k_stride_head = k.stride(0), k.stride(1), k.stride(2)
+    a.v_stride_page, a.v_stride_slot, a.v_stride_head = v.stride(0), v.stride(1), v.stride(2)
+    if k_scale is not None:
+        a.scale_stride_page, a.scale_stride_head = k_scale.stride(0), k_scale.stride(1)
+    a.page_table_stride = table.stride(0)
+    a.batch, a.groups = q.shape[0], prefix_lens.shape[0]
+    a.num_heads, a.num_kv_heads, a.head_dim = q.shape[-2], k.shape[2], q.shape[-1]
+    a.page_size, a.num_pages, a.max_pages = cache.page_size, k.shape[0], table.shape[1]
+    a.q_dtype, a.kv_dtype = dtype_code(q.dtype), dtype_code(k.dtype)
+    a.softmax_scale = float(softmax_scale)
+    return a
+
+
+def shared_workspace_bytes(rows: int, num_heads: int, head_dim: int, splits: int) -> int:
+    return int(lib().fat_paged_decode_shared_workspace_bytes(rows, num_heads, head_dim, splits))
+
+
+def shared_with_args(a: SharedArgs, workspace: torch.Tensor, stream: int) -> None:
+    """Enqueue ``fat_paged_decode_shared`` with a prepared argument block."""
+    a.workspace = _ptr(workspace)
+    a.workspace_bytes = workspace.numel() * workspace.element_size()
+    _check(lib().fat_paged_decode_shared(ctypes.byref(a), _c_vp(stream)), "fat_paged_decode_shared")
 
 
 # FAT_DECODE_NOALLOC_MAX_WORKSPACE of include/fat_abi.h

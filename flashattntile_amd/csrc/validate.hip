@@ -121,6 +121,7 @@ struct CheckParams {
   const int32_t* ids[3];
   int32_t* scratch;
   int32_t num_pages;
+  int32_t tokens;
 };
 
 struct RMin { template <typename T> static __device__ __forceinline__ T f(T a, T b) { return a < b ? a : b; } };
@@ -266,6 +267,105 @@ __global__ __launch_bounds__(kCheckThreads) void check_kernel(const CheckParams 
   }
 }
 
+// SHARED: workgroup x takes rows x, x + gridDim.x, ..: the page range of their
+// used columns, and whether those that the prefix fills name the pages of the
+// group's first row (else INT_MIN for the smallest id).  Workgroup 0 also
+// reduces lengths, offsets and prefixes.
+__global__ __launch_bounds__(kCheckThreads) void check_shared_kernel(const CheckParams p) {
+  const int tid = threadIdx.x;
+  const int G = (int)p.count;
+  const int32_t* prefix = p.ids[0];
+  auto group_of = [&](int b) {  // the largest g with cu_q[g] <= b, -1: none
+    int lo = -1, hi = G;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.cu_q[mid] <= b) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  auto put = [&](int word, long long v) {
+    __hip_atomic_store(p.host + word, (int64_t)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  };
+  int pmn = INT_MAX, pmx = INT_MIN;
+  bool differs = false;
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {  // uniform
+    const int g = group_of(b);
+    const int lead = g < 0 ? b : max(p.cu_q[g], 0);
+    const long long len = max(p.lens[b], 0);
+    const int cols = (int)min((len + p.P - 1) / p.P, (long long)p.max_pages);
+    const int same = lead == b ? 0 : min(max(prefix[g], 0) / p.P, cols);
+    const int32_t* row = p.pt + b * p.pt_sb;
+    const int32_t* first = p.pt + lead * p.pt_sb;
+#pragma unroll 4
+    for (int c = tid; c < cols; c += kCheckThreads) {
+      const int id = row[c];
+      pmn = min(pmn, id);
+      pmx = max(pmx, id);
+      if (c < same) differs |= first[c] != id;
+    }
+  }
+  pmn = (int)check_reduce<RMin>(differs ? INT_MIN : pmn);
+  pmx = (int)check_reduce<RMax>(pmx);
+  if (blockIdx.x == 0) {  // uniform
+    long long mn = INT_MAX, mx = INT_MIN, pages = 0, flags = 0, most = 0, longest = 0, behind = 0, sum_p = 0,
+              sum_own = 0, sum_rows = 0;
+    for (int b = tid; b < p.B; b += kCheckThreads) {
+      const long long len = p.lens[b];
+      const int g = group_of(b);
+      const long long n = g < 0 ? 0 : prefix[g];
+      mn = min(mn, len);
+      mx = max(mx, len);
+      pages += (max(len, 0ll) + p.P - 1) / p.P;
+      if (n > len - p.tokens + 1) flags |= 4;
+      behind = max(behind, len - n);
+      sum_own += len - n;
+    }
+    for (int g = tid; g < G; g += kCheckThreads) {
+      const long long seqs = (long long)p.cu_q[g + 1] - p.cu_q[g];
+      flags |= (seqs < 0 ? 1 : 0) | (prefix[g] < 0 ? 2 : 0);
+      most = max(most, seqs);
+      if (seqs > 0) {
+        longest = max(longest, (long long)prefix[g]);
+        sum_p += prefix[g];
+        sum_rows += prefix[g] * seqs;
+      }
+    }
+    mn = check_reduce<RMin>(mn);
+    mx = check_reduce<RMax>(mx);
+    pages = check_reduce<RSum>(pages);
+    flags = check_reduce<ROr>(flags);
+    most = check_reduce<RMax>(most);
+    longest = check_reduce<RMax>(longest);
+    behind = check_reduce<RMax>(behind);
+    sum_p = check_reduce<RSum>(sum_p);
+    sum_own = check_reduce<RSum>(sum_own);
+    sum_rows = check_reduce<RSum>(sum_rows);
+    if (tid == 0) {
+      put(0, mn);
+      put(1, mx);
+      put(2, pages);
+      put(3, p.cu_q[0]);
+      put(4, p.cu_q[G]);
+      put(5, most);
+      put(6, longest);
+      put(7, flags);
+      put(8, behind);
+      put(9, sum_p);
+      put(10, sum_own);
+      put(11, sum_rows);
+    }
+  }
+  if (tid == 0) {
+    const int at = FAT_CHECK_RESULTS + 2 * blockIdx.x;
+    put(at, (long long)(((unsigned long long)(uint32_t)pmx << 32) | (uint32_t)pmn));
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the results are complete
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    put(at + 1, p.ticket);
+  }
+}
+
 // COPY and FORK: ranges, and ids that are given twice or on both sides.  An id
 // d of list b is "owned" by the last writer of own[d], and own needs no
 // clearing: own[x] names an element k only if 0 <= k < count and b[k] == x, so
@@ -359,25 +459,28 @@ int check_groups(const fat_check_args* a) {
   if (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_APPEND || a->kind == FAT_CHECK_COPY ||
       a->kind == FAT_CHECK_FORK)
     return 1;
+  if (a->kind == FAT_CHECK_SHARED) return std::min(a->batch, FAT_CHECK_MAX_GROUPS);
   const int64_t entries = a->kind == FAT_CHECK_RANGE ? a->count : (int64_t)a->batch * a->max_pages;
   const int64_t n = (entries + fat::kCheckEntries - 1) / fat::kCheckEntries;
   return (int)std::min<int64_t>(std::max<int64_t>(n, 1), FAT_CHECK_MAX_GROUPS);
 }
 
 bool check_args_ok(const fat_check_args* a, const char* who) {
-  const bool cu = a && (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_PAGED);
+  const bool shared = a && a->kind == FAT_CHECK_SHARED;
+  const bool cu = a && (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_PAGED || shared);
   const bool range = a && a->kind == FAT_CHECK_RANGE;
   const bool copy = a && a->kind == FAT_CHECK_COPY, fork = a && a->kind == FAT_CHECK_FORK;
   const bool lens = a && a->kind != FAT_CHECK_VARLEN && !range && !copy;
-  const bool ids = copy || fork || (a && a->kind == FAT_CHECK_FREE && a->count > 0);
+  const bool ids = copy || fork || shared || (a && a->kind == FAT_CHECK_FREE && a->count > 0);
   if (!a || !a->host || (ids && !a->ids[0]) || ((copy || fork) && (!a->ids[1] || !a->scratch)) ||
       (fork && !a->ids[2]) || (cu && !a->cu_q) || (a->kind == FAT_CHECK_VARLEN && !a->cu_k) || (lens && !a->seq_lens) ||
       (lens && !a->page_table) || (range && !a->values)) {
     fat_host::set_error("%s: a required pointer is NULL", who);
     return false;
   }
-  if (a->kind < FAT_CHECK_CACHE || a->kind > FAT_CHECK_FREE || (!range && !copy && a->batch <= 0) ||
+  if (a->kind < FAT_CHECK_CACHE || a->kind > FAT_CHECK_SHARED || (!range && !copy && a->batch <= 0) ||
       a->ticket <= 0 || (range && a->count <= 0) || (a->kind == FAT_CHECK_FREE && a->count < 0) ||
+      (shared && (a->count <= 0 || a->count > INT_MAX || a->tokens <= 0)) ||
       ((copy || fork) && (a->count <= 0 || a->count > INT_MAX || a->num_pages <= 0)) ||
       (lens && (a->max_pages <= 0 || a->page_size <= 0 || a->page_table_stride < 0)) ||
       (a->kind == FAT_CHECK_CACHE && a->page_table_stride < a->max_pages)) {
@@ -405,7 +508,7 @@ extern "C" int fat_check_begin(const fat_check_args* a, void* stream_ptr) {
   }
   const fat::CheckParams prm{a->cu_q, a->cu_k, a->seq_lens, a->page_table, a->page_table_stride, a->host,
                              a->ticket, a->batch, a->max_pages, a->page_size, a->values, a->count,
-                             {a->ids[0], a->ids[1], a->ids[2]}, a->scratch, a->num_pages};
+                             {a->ids[0], a->ids[1], a->ids[2]}, a->scratch, a->num_pages, a->tokens};
   const dim3 grid((unsigned)check_groups(a)), block(fat::kCheckThreads);
   switch (a->kind) {
     case FAT_CHECK_CACHE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_CACHE>), grid, block, 0, stream, prm); break;
@@ -413,6 +516,7 @@ extern "C" int fat_check_begin(const fat_check_args* a, void* stream_ptr) {
     case FAT_CHECK_PAGED: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_PAGED>), grid, block, 0, stream, prm); break;
     case FAT_CHECK_RANGE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_RANGE>), grid, block, 0, stream, prm); break;
     case FAT_CHECK_FREE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_FREE>), grid, block, 0, stream, prm); break;
+    case FAT_CHECK_SHARED: hipLaunchKernelGGL(fat::check_shared_kernel, grid, block, 0, stream, prm); break;
     case FAT_CHECK_COPY:
       hipLaunchKernelGGL((fat::check_lists_kernel<FAT_CHECK_COPY>), grid, dim3(fat::kListThreads), 0, stream, prm);
       break;
@@ -470,6 +574,10 @@ extern "C" int fat_check_wait(const fat_check_args* a, void* stream_ptr, int64_t
     const bool nan = lo == INT_MIN && hi == INT_MAX;
     lo = nan ? 0x7fc00000 : lo ^ ((lo >> 31) & 0x7fffffff);
     hi = nan ? 0x7fc00000 : hi ^ ((hi >> 31) & 0x7fffffff);
+  }
+  if (a->kind == FAT_CHECK_SHARED && lo == INT_MIN) {
+    result[7] |= 8;
+    lo = 0;
   }
   result[12] = lo;
   result[13] = hi;

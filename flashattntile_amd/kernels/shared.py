@@ -1,0 +1,257 @@
+"""Decode of sequences that share a prefix: host side of ``csrc/decode_shared.hip``.
+
+:func:`paged_decode_attention_shared` computes what
+:func:`~flashattntile_amd.kernels.decode.paged_decode_attention`, its 8-bit and
+its multi-token forms compute, for a batch whose sequences come in groups with
+the same first keys (a system prompt, the samples of one prompt, questions about
+one document): those keys are read once for all queries of the group instead of
+once per sequence (the reference has no counterpart; its decode reads every
+sequence's own table, ``kernels/decode.py:47-127``).
+
+:func:`paged_decode_shared_launch` is the sync-free entry below the validation.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _hip
+from ..paging import PagedKVCache, _check_layout
+from .decode import (_QUANT_DTYPES, _decode, _dense_scales, _require_rocm, _resolve_config, _scale_of)
+
+__all__ = ["paged_decode_attention_shared", "paged_decode_shared_launch", "shared_splits"]
+
+# Partials of a launch: prefix_split chunks of prefix_chunk keys of a group's
+# prefix, split chunks of chunk keys of a sequence's own; None: shared_splits.
+_CONFIG_KEYS = ("prefix_split", "split")
+
+
+def _check_inputs(q, cache: PagedKVCache, cu_groups, prefix_lens, scales) -> None:
+    """The host-only checks."""
+    if not isinstance(cache, PagedKVCache):
+        raise TypeError("cache must be a PagedKVCache")
+    _check_layout(cache)
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q must be [batch, heads, head_dim] or [batch, q_len, heads, head_dim], got {tuple(q.shape)}")
+    if q.shape[0] != cache.batch_size:
+        raise ValueError(f"q batch {q.shape[0]} != cache batch {cache.batch_size}")
+    if q.shape[-1] != cache.head_dim:
+        raise ValueError(f"q head_dim {q.shape[-1]} != cache head_dim {cache.head_dim}")
+    if q.shape[-2] % cache.num_kv_heads != 0:
+        raise ValueError(f"num_heads {q.shape[-2]} must be divisible by num_kv_heads {cache.num_kv_heads}")
+    if q.dim() == 4 and not 1 <= q.shape[1] <= 64:
+        raise ValueError(f"multi-token decode takes 1 to 64 tokens per sequence, got {q.shape[1]}")
+    for name, t in (("cu_groups", cu_groups), ("prefix_lens", prefix_lens)):
+        if t.dim() != 1 or t.dtype != torch.int32:
+            raise ValueError(f"{name} must be a 1-D int32 tensor")
+    if cu_groups.shape[0] != prefix_lens.shape[0] + 1 or prefix_lens.shape[0] == 0:
+        raise ValueError(f"cu_groups must have one entry more than prefix_lens, at least two; got "
+                         f"{cu_groups.shape[0]} and {prefix_lens.shape[0]}")
+    if any(t.device != q.device for t in (cache.k_cache, cache.page_table, cache.seq_lens, cu_groups, prefix_lens)):
+        raise ValueError("q, the cache, its page table, seq_lens, cu_groups and prefix_lens must live on one device")
+    quantized = cache.k_cache.dtype in _QUANT_DTYPES
+    if quantized != (scales is not None):
+        raise ValueError("an int8/float8 cache needs scales, and only such a cache takes them")
+    if quantized:
+        if q.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"quantised decode requires fp16/bf16 queries, got {q.dtype}")
+        k_scale = scales["k"] if isinstance(scales, dict) else scales.k
+        v_scale = scales["v"] if isinstance(scales, dict) else scales.v
+        expected = (cache.num_pages, cache.num_kv_heads)
+        if tuple(k_scale.shape) != expected or tuple(v_scale.shape) != expected:
+            raise ValueError(f"scales must have shape {expected}, got {tuple(k_scale.shape)}")
+        if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+            raise ValueError("scales must be float32")
+        if k_scale.device != q.device or v_scale.device != q.device:
+            raise ValueError("scales must live on q's device")
+    elif cache.k_cache.dtype != q.dtype:
+        raise ValueError(f"q dtype {q.dtype} must match cache dtype {cache.k_cache.dtype}")
+
+
+def _assess(r: list[int], q, cache: PagedKVCache) -> None:
+    """The device-side checks on their numbers (``FAT_CHECK_SHARED``)."""
+    tokens = q.shape[1] if q.dim() == 4 else 1
+    flags = r[7]
+    if r[3] != 0:
+        raise ValueError("cu_groups must start at 0")
+    if flags & 1:
+        raise ValueError("cu_groups must be non-decreasing")
+    if r[4] != cache.batch_size:
+        raise ValueError(f"cu_groups must end at the batch size {cache.batch_size}, got {r[4]}")
+    if flags & 2:
+        raise ValueError("prefix_lens must be non-negative")
+    if r[0] < 0:
+        raise AssertionError("seq_lens must be non-negative")
+    if r[1] > cache.capacity:
+        raise AssertionError(f"seq_len {r[1]} exceeds page-table capacity {cache.capacity}")
+    if r[0] < tokens:
+        raise ValueError(f"decode requires every sequence to hold its {tokens} new token(s) (shortest seq_len {r[0]})")
+    if flags & 4:
+        raise ValueError("a group's prefix must be no longer than what the first new token of each of its sequences "
+                         "sees (prefix_lens[g] <= seq_lens[b] - q_len + 1)")
+    if flags & 8:
+        raise ValueError("the sequences of a group must share the pages that its prefix fills")
+    if r[12] < 0:
+        raise AssertionError("page_table contains a negative page id")
+    if r[13] >= cache.num_pages:
+        raise AssertionError(f"page_table references page {r[13]} but cache has {cache.num_pages} pages")
+
+
+def _takes(q, cache: PagedKVCache) -> bool:
+    """Whether the shared-prefix kernel takes the launch."""
+    k, v = cache.k_cache, cache.v_cache
+    if q.dtype not in (torch.float16, torch.bfloat16) or cache.head_dim not in (64, 128):
+        return False
+    if cache.capacity > 2 ** 31 - 4097:
+        return False
+    eb = k.element_size()
+    words = [k.data_ptr(), v.data_ptr(), q.data_ptr()]
+    words += [eb * s for t in (k, v) for s in t.stride()[:3]]
+    return all(x % 16 == 0 for x in words)
+
+
+def _up(n: int, to: int) -> int:
+    return -(-n // to) * to
+
+
+def shared_splits(rows: int, num_kv_heads: int, groups: int, max_prefix: int, max_own: int, batch: int,
+                  own_tiles: int, max_group_rows: int) -> dict:
+    """Partials of a launch: ``prefix_split`` x ``prefix_chunk`` keys of every
+    prefix, ``split`` x ``chunk`` own keys of every sequence."""
+    tiles = -(-max_group_rows // 32)
+    per_split = max(1, groups * num_kv_heads * tiles)
+    prefix_split = max(1, min(512 // per_split, 32, -(-max_prefix // 256)))
+    own = max(1, batch * num_kv_heads * own_tiles)
+    split = max(1, min(512 // own, 16, -(-max_own // 256)))
+    return _chunks(prefix_split, split, max_prefix, max_own)
+
+
+def _chunks(prefix_split: int, split: int, max_prefix: int, max_own: int) -> dict:
+    return {"prefix_split": prefix_split, "prefix_chunk": _up(max(1, -(-max_prefix // prefix_split)), 32),
+            "split": split, "chunk": _up(max(1, -(-max_own // split)), 32)}
+
+
+def _block(q, cache, cu_groups, prefix_lens, scale, scales, out=None):
+    """The argument block but for its splits, its output, and what has to live
+    until the launch is enqueued."""
+    if cache.k_cache.stride(-1) != 1 or cache.v_cache.stride(-1) != 1:
+        raise ValueError("k_cache and v_cache need a contiguous head_dim axis")
+    if out is None:
+        out = torch.empty_like(q)
+    pt = cache.page_table if cache.page_table.stride(-1) == 1 else cache.page_table.contiguous()
+    sl, cu, pre = cache.seq_lens.contiguous(), cu_groups.contiguous(), prefix_lens.contiguous()
+    dense = PagedKVCache(cache.k_cache, cache.v_cache, pt, sl, cache.page_size)
+    sc = None if scales is None else _dense_scales(scales)
+    a = _hip.shared_args(q, dense, cu, pre, out, scale, *((sc["k"], sc["v"]) if sc else ()))
+    return a, out, (q, dense, cu, pre, sc)
+
+
+def _launch(a, q, cfg: dict, max_group: int, workspace=None) -> None:
+    rows = q.shape[0] * (q.shape[1] if q.dim() == 4 else 1)
+    # fat_paged_decode_shared_workspace_bytes: (acc, m, l) per (query row, head, partial)
+    need = 4 * rows * q.shape[-2] * (cfg["prefix_split"] + cfg["split"]) * (q.shape[-1] + 2)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    a.max_group = max_group
+    a.prefix_split, a.prefix_chunk = cfg["prefix_split"], cfg["prefix_chunk"]
+    a.split, a.chunk = cfg["split"], cfg["chunk"]
+    _hip.shared_with_args(a, workspace, _hip.current_stream_handle(q.device))
+
+
+def _own_tiles(q, cache: PagedKVCache) -> int:
+    tokens = q.shape[1] if q.dim() == 4 else 1
+    return -(-(tokens * q.shape[-2] // cache.num_kv_heads) // 32)
+
+
+def paged_decode_shared_launch(q: torch.Tensor, cache: PagedKVCache, cu_groups: torch.Tensor,
+                               prefix_lens: torch.Tensor, softmax_scale: float, max_prefix: int, max_own: int,
+                               max_group: int | None = None, out: torch.Tensor | None = None,
+                               workspace: torch.Tensor | None = None, scales=None,
+                               config: dict | None = None) -> torch.Tensor:
+    """Enqueue the shared-prefix decode without validation or synchronisation
+    (capture, serving loops that validated once).
+
+    ``max_prefix`` and ``max_own`` bound the groups' prefixes and the keys
+    behind them, ``max_group`` the sequences of a group (default: the batch);
+    they size the grid, and more keys than they say are still attended.
+    Lengths, table, groups and prefixes are read on the device at every run.
+    ``q`` must be contiguous; ``out`` and ``workspace`` (uint8, 4 x rows x heads
+    x partials x (head_dim + 2) bytes) may be passed in to avoid allocations.
+    Takes fp16/bf16 queries at head_dim 64 or 128, else raises.
+    """
+    a, out, _keep = _block(q, cache, cu_groups, prefix_lens, softmax_scale, scales, out)
+    cfg = _resolve(config, q, cache, prefix_lens.shape[0], max_prefix, max_own, max_group or q.shape[0])
+    _launch(a, q, cfg, max_group or q.shape[0], workspace)
+    return out
+
+
+def _resolve(config, q, cache, groups: int, max_prefix: int, max_own: int, max_group: int) -> dict:
+    per_seq = (q.shape[1] if q.dim() == 4 else 1) * q.shape[-2] // cache.num_kv_heads
+    cfg = shared_splits(q.shape[0] * per_seq, cache.num_kv_heads, groups, max_prefix, max_own, q.shape[0],
+                        _own_tiles(q, cache), max_group * per_seq)
+    if config is None:
+        return cfg
+    unknown = set(config) - set(_CONFIG_KEYS)
+    if unknown:
+        raise ValueError(f"unknown shared decode config keys: {sorted(unknown)}")
+    given = {k: v for k, v in config.items() if v is not None}
+    for k, v in given.items():
+        if not isinstance(v, int) or isinstance(v, bool) or not 1 <= v <= 64:
+            raise ValueError(f"{k} must be an integer in [1, 64], got {v}")
+    return _chunks(given.get("prefix_split", cfg["prefix_split"]), given.get("split", cfg["split"]), max_prefix,
+                   max_own)
+
+
+def paged_decode_attention_shared(
+    q: torch.Tensor,
+    cache: PagedKVCache,
+    cu_groups: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    softmax_scale: float | None = None,
+    config: dict | None = None,
+    scales=None,
+) -> torch.Tensor:
+    """Paged decode of groups of sequences with the same first keys.
+
+    ``q``: ``[batch, heads, head_dim]`` or, multi-token, ``[batch, q_len, heads,
+    head_dim]``, as :func:`paged_decode_attention` and ``..._multi`` take it.
+    ``cu_groups`` (int32 ``[groups + 1]``, from 0 to batch): sequences
+    ``cu_groups[g] .. cu_groups[g + 1] - 1`` are group g.  ``prefix_lens`` (int32
+    ``[groups]``): the keys they share, read through the table row of the
+    group's first sequence; ``seq_lens`` counts them too.  A prefix of 0 and
+    groups of one sequence are valid; one that ends inside a page too (every
+    sequence then has its own copy of that page, as
+    :func:`~flashattntile_amd.page_ops.fork_sequences` makes it), the pages it
+    fills must be the same ids in all rows of the group.  ``scales`` selects an
+    int8 / float8_e4m3fn cache.  ``config``: ``prefix_split`` and ``split``,
+    partials per prefix and per sequence (default: by the lengths).
+
+    Shapes that the kernel isn't built for (fp32, other head_dims than 64 and
+    128, rows that aren't 16-byte aligned) run as ordinary decode, which reads
+    the prefix once per sequence.  Returns ``q``'s shape and dtype.
+    """
+    _check_inputs(q, cache, cu_groups, prefix_lens, scales)
+    _require_rocm(q, cache, "paged_decode_attention_shared")
+    if cache.batch_size == 0 or cache.page_table.numel() == 0:
+        raise ValueError("decode requires every sequence to hold at least one cached token")
+    tokens = q.shape[1] if q.dim() == 4 else 1
+    scale = _scale_of(q, softmax_scale)
+    q = q.contiguous()
+    device = q.device
+    stream = _hip.current_stream_handle(device)
+    sl, pt = cache.seq_lens.contiguous(), cache.page_table
+    pt = pt if pt.stride(-1) == 1 else pt.contiguous()
+    check = _hip.check_begin(_hip.CHECK_SHARED, stream, device, cu_q=cu_groups.contiguous(), seq_lens=sl, page_table=pt,
+                             page_size=cache.page_size, ids=(prefix_lens.contiguous(),), tokens=tokens)
+    # prepared while the check kernel runs
+    block = _block(q, cache, cu_groups, prefix_lens, scale, scales) if _takes(q, cache) else None
+    r = check.wait()
+    _assess(r, q, cache)
+    if block is None:
+        cfg = _resolve_config(None, q, cache, r[1], r[2], q_len=tokens)
+        return _decode(q, cache, scale, cfg, None, None if scales is None else _dense_scales(scales))
+    a, out, keep = block
+    cfg = _resolve(config, q, cache, prefix_lens.shape[0], r[6], r[8], max(1, r[5]))
+    _launch(a, q, cfg, max(1, r[5]))
+    del keep
+    return out

@@ -46,7 +46,8 @@
 extern "C" {
 #endif
 
-/* 18: operations on pages (fat_copy_pages, fat_fork_sequences,
+/* 19: fat_paged_decode_shared and FAT_CHECK_SHARED.
+ * 18: operations on pages (fat_copy_pages, fat_fork_sequences,
  *     fat_free_sequences, fat_compact_pages) and FAT_CHECK_COPY, _FORK, _FREE.
  * 17: fat_decode_args.workspace_bytes; fat_stream_capture_id.
  * 16: fat_prefill_paged_args.v_workspace, .total_k and fat_prefill_paged_v_bytes:
@@ -70,7 +71,7 @@ extern "C" {
  * 8: fp32 decode, any page size and head_dim 32/256 through the generic
  *    decode kernel (FAT_KERNEL_DECODE_GENERIC); the paged prefill `rows`
  *    field replaces the library's environment overrides. */
-#define FAT_ABI_VERSION 18
+#define FAT_ABI_VERSION 19
 
 /* Element types understood by the kernels. */
 enum fat_dtype {
@@ -510,6 +511,69 @@ int fat_quantize_pages(const fat_quantize_args* args, void* stream);
 int fat_append_kv(const fat_append_args* args, void* stream);
 
 /*
+ * Paged decode of groups of sequences that share a prefix (no reference
+ * counterpart: fat_paged_decode's function, with the shared keys read once for
+ * all sequences of a group).
+ * Sequences cu_groups[g] .. cu_groups[g + 1] - 1 are group g (cu_groups[0] = 0,
+ * non-decreasing, cu_groups[groups] = batch); their first prefix_lens[g] keys
+ * are the same, and are read through the table row of the group's first
+ * sequence.  seq_lens counts all keys, the shared ones among them; prefix_lens[g]
+ * <= seq_lens[b] - q_len + 1.  A prefix of 0 keys and groups of one or no
+ * sequence are valid.  Layouts, q_len and 8-bit caches as for fat_paged_decode;
+ * fp16/bf16 queries, head_dim 64 or 128, any page size (FAT_E_UNSUPPORTED
+ * otherwise), 16-byte aligned q, K, V and workspace rows.  Lengths, offsets and
+ * page ids are clamped on the device: bad ones give wrong answers, never an
+ * access out of bounds.
+ * The shared keys are cut into prefix_split partials of prefix_chunk keys, a
+ * sequence's own into split partials of chunk keys (multiples of 32; the last
+ * takes any keys beyond), joined by log-sum-exp through `workspace`, which holds
+ * fat_paged_decode_shared_workspace_bytes(batch * q_len, num_heads, head_dim,
+ * prefix_split + split) bytes.  Launches that may run at the same time need one
+ * each.  max_group: an upper bound of the sequences of a group.
+ */
+typedef struct fat_shared_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_groups;   /* [groups + 1] */
+  const int32_t* prefix_lens; /* [groups] */
+  void* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  int64_t k_stride_page, k_stride_slot, k_stride_head;
+  int64_t v_stride_page, v_stride_slot, v_stride_head;
+  int64_t scale_stride_page, scale_stride_head;
+  int64_t page_table_stride;
+  int64_t out_stride_b, out_stride_t, out_stride_h;
+  int32_t batch;
+  int32_t groups;
+  int32_t max_group;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t max_pages;
+  int32_t q_len; /* 0 or 1: one query per sequence, the token strides are ignored */
+  int32_t q_dtype;
+  int32_t kv_dtype;
+  int32_t prefix_split, prefix_chunk;
+  int32_t split, chunk;
+  float softmax_scale;
+} fat_shared_args;
+
+size_t fat_paged_decode_shared_workspace_bytes(int32_t rows, int32_t num_heads,
+                                               int32_t head_dim, int32_t splits);
+
+/* Enqueue shared-prefix decode on `stream`. */
+int fat_paged_decode_shared(const fat_shared_args* args, void* stream);
+
+/*
  * Operations on the pages of a cache (no reference counterpart: its engine
  * neither shares pages nor moves them).
  *
@@ -664,6 +728,9 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *        FAT_CHECK_FORK    parents, children and pages = ids[0 .. 2], `count`
  *                          each, with seq_lens and the page table
  *        FAT_CHECK_FREE    FAT_CHECK_CACHE, and rows = ids[0], `count` of them
+ *        FAT_CHECK_SHARED  FAT_CHECK_CACHE, and the groups cu_q [count + 1] with
+ *                          the prefixes ids[0] [count]; tokens = queries per
+ *                          sequence
  *   host   int64 [FAT_CHECK_HOST_WORDS]: page-locked host memory that the
  *          device can write, zero before its first use and used by one call
  *          at a time
@@ -688,7 +755,14 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *          child that is a parent too, 16 a child that holds tokens, 32 a
  *          parent longer than the table or negative, and of parents that end
  *          inside a page: 64 that page, 128 pages[i] out of [0, num_pages),
- *          256 pages[i] given twice
+ *          256 pages[i] given twice; SHARED: 1 cu_q decreases, 2 a negative
+ *          prefix, 4 one beyond seq_lens - tokens + 1 of a sequence of its
+ *          group, 8 a sequence whose table row names other pages than the
+ *          group's first where the prefix fills pages.  SHARED also: 3, 4
+ *          cu_q[0], cu_q[count]; 5 the most sequences of a group; 6 the longest
+ *          prefix (of a group with sequences); 8 the most keys behind the prefix;
+ *          9 sum over groups of prefix; 10 sum over sequences of the keys behind
+ *          it; 11 sum over groups of prefix x sequences
  * Entries that a kind doesn't name are undefined.  `scratch` (COPY: int32
  * [num_pages], FORK: int32 [num_pages + batch], device memory) need not be
  * cleared and holds nothing afterwards.
@@ -701,7 +775,8 @@ enum fat_check_kind {
   FAT_CHECK_RANGE = 4,
   FAT_CHECK_COPY = 5,
   FAT_CHECK_FORK = 6,
-  FAT_CHECK_FREE = 7
+  FAT_CHECK_FREE = 7,
+  FAT_CHECK_SHARED = 8
 };
 #define FAT_CHECK_RESULTS 16
 #define FAT_CHECK_MAX_GROUPS 64
@@ -723,6 +798,7 @@ typedef struct fat_check_args {
   const int32_t* ids[3]; /* [count] each: COPY, FORK and FREE only */
   int32_t* scratch;
   int32_t num_pages; /* COPY and FORK only */
+  int32_t tokens;    /* SHARED only */
 } fat_check_args;
 
 /* Enqueue the check on `stream`.  FAT_E_LAUNCH while the stream is capturing
