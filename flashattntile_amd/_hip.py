@@ -335,6 +335,7 @@ class SharedArgs(ctypes.Structure):
         ("prefix_chunk", _c_i32),
         ("split", _c_i32),
         ("chunk", _c_i32),
+        ("row_blocks", _c_i32),
         ("softmax_scale", ctypes.c_float),
     ]
 

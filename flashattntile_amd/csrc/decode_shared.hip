@@ -43,13 +43,22 @@ struct SharedParams {
   float* ws_acc;  // [B * T * H, S, D]
   float* ws_ml;   // [B * T * H, S, 2]
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
-  int64_t k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;  // bytes
-  int64_t sc_sp, sc_sh;
+  int64_t k_sh, v_sh;               // bytes
+  uint32_t k_sp, k_ss, v_sp, v_ss;  // bytes; a page is below 4 GiB
+  int64_t sc_sh;
+  uint32_t sc_sp;
   int64_t pt_sb;
   int32_t B, G, T, H, Hkv, group;
-  int32_t P, log2P, num_pages, max_pages;
-  uint32_t invP;
-  float scale_log2;
+  int32_t P, num_pages, max_pages;
+  uint32_t invP;  // floor(2^32 / P), 2^32 - 1 for P = 1: floor(t / P) is the high product of t, or one more
+  // Columns and slots that a key group's next tile lies behind its last one
+  // (32 KG tokens), for prefix items and own items.
+  uint32_t step_col[2], step_slot[2];
+  float scale_log2;  // > 0 (or NaN)
+  // Applied to every Q dword as it is loaded, (q & q_and) ^ q_xor: a negative
+  // softmax scale runs as its absolute value with Q's signs flipped (exact), a
+  // zero one with Q zeroed.  Identity: ~0u, 0.
+  uint32_t q_and, q_xor;
   int32_t tiles;                     // row tiles of the largest group
   int32_t prefix_split, prefix_chunk;  // partials and keys of each
   int32_t split, chunk;
@@ -73,6 +82,38 @@ __device__ __forceinline__ int group_of(const int32_t* cu, int G, int b) {
   return lo;
 }
 
+// (Not as inline asm: it would read the MFMA's results without the wait states
+// that the compiler puts in front of an instruction it knows.)
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// 16 int8 or e4m3 codes as their exact values in QT (8 packed pairs).
+template <typename QT, int KV>
+__device__ __forceinline__ void codes_exact(const u32x4& raw, u32 (&o)[8]) {
+  constexpr bool H = std::is_same<QT, F16>::value;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (KV == KV_FP8 && H) {
+      o[2 * j] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[j], 1.0f, false));
+      o[2 * j + 1] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[j], 1.0f, true));
+    } else if constexpr (KV == KV_FP8) {
+      o[2 * j] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j], 1.0f, false));
+      o[2 * j + 1] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j], 1.0f, true));
+    } else if constexpr (H) {
+      // fp16 bits 0x6400 | u are 1024 + u exactly (u = x + 128, the byte with its
+      // sign bit flipped); adding -1152 leaves x.
+      const u32 u = raw[j] ^ 0x80808080u;
+      const f16x2 bias = {(f16)-1152.0f, (f16)-1152.0f};
+      o[2 * j] = __builtin_bit_cast(u32, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias);
+      o[2 * j + 1] = __builtin_bit_cast(u32, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias);
+    } else {
+      float f[4];
+      i8x4_biased(raw[j], f);
+      o[2 * j] = Pair<QT>::pack(f[0] - 128.0f, f[1] - 128.0f);
+      o[2 * j + 1] = Pair<QT>::pack(f[2] - 128.0f, f[3] - 128.0f);
+    }
+  }
+}
+
 template <typename QT, int KV, int D, int RB>
 struct SharedTile {
   static constexpr int KG = kSharedWaves / RB;
@@ -89,8 +130,15 @@ struct SharedTile {
   static constexpr int NLD = NCH > NT ? NCH / NT : 1;  // per lane
   static constexpr int OS = D + 4;               // row stride (floats) of the key groups' join
   static constexpr int kTile = 32 * (K_RS + V_RS);  // elements
-  static constexpr bool FOLD = KV != KV_SAME && std::is_same<QT, F16>::value;  // k_scale on the scores
-  static constexpr int kTileBytes = KG * kBufs * kTile * 2 + (FOLD ? KG * kBufs * 32 * 4 : 0);
+  // 8-bit caches: the codes are staged as they are (exact in fp16 and bf16) and
+  // k_scale multiplies the fp32 scores.  v_scale multiplies P for bf16, whose
+  // exponents hold any scale; in fp16 the P of a page with a small scale would
+  // lose its bits beside one with a large scale, so V is staged as
+  // round_to_fp16(x * scale) there.
+  static constexpr bool FOLD = KV != KV_SAME;
+  static constexpr bool FOLD_V = FOLD && std::is_same<QT, BF16>::value;
+  static constexpr int kScaleFloats = FOLD_V ? 64 : FOLD ? 32 : 0;  // of a tile's keys: K's, V's
+  static constexpr int kTileBytes = KG * kBufs * (kTile * 2 + kScaleFloats * 4);
   static constexpr int kJoinBytes = KG > 1 ? (kSharedWaves * 32 * OS + kSharedWaves * 32 * 2) * 4 : 0;
   static constexpr int kBytes = kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes;
 };
@@ -104,7 +152,7 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   using Tl = SharedTile<QT, KV, D, RB>;
   constexpr int KG = Tl::KG, KS = Tl::KS, DB = Tl::DB, K_RS = Tl::K_RS, V_RS = Tl::V_RS, EPC = Tl::EPC, CPR = Tl::CPR,
                 NT = Tl::NT, NCH = Tl::NCH, NLD = Tl::NLD, OS = Tl::OS;
-  constexpr bool FOLD = Tl::FOLD;
+  constexpr bool FOLD = Tl::FOLD, FOLD_V = Tl::FOLD_V;
   // P enters the second product as bf16 hi + lo parts: one bf16 alone (2^-9) would
   // show beside the output's own rounding where a row sees few keys.
   constexpr bool SPLIT_P = std::is_same<QT, BF16>::value;
@@ -136,12 +184,13 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   {
     const uint8_t* qp = p.q + 2 * ((int64_t)my_b * p.q_sb + (int64_t)my_t * p.q_st + (int64_t)my_h * p.q_sh + 8 * g);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + 32 * ks);
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = (*reinterpret_cast<const u32x4*>(qp + 32 * ks) & p.q_and) ^ p.q_xor;
   }
 
   // Staging: chunk i NT + st of a tile is this lane's, st its place in the key group.
-  const int st = rb * 64 + lane;
-  const bool stages = NCH >= NT || st < NCH;
+  // (Where a tile has fewer chunks than lanes, the others load what lane st loads.)
+  const int st = (rb * 64 + lane) % NCH;
+  const bool stages = NCH >= NT || rb * 64 + lane < NCH;
   const int srow = st / CPR;  // row of chunk 0; chunk i's is srow + i NT / CPR
   const int scol = st % CPR;
   const uint8_t* const kh = p.k + (int64_t)kvh * p.k_sh + 16 * scol;
@@ -151,90 +200,152 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   struct Raw {
     u32x4 k[NLD], v[NLD];
     float ksc[NLD], vsc[NLD];
-  } R0;
-  int pid[NLD], pslot[NLD];
-  // Page id and slot of this lane's rows of tile t; rows behind the end look up
-  // its last key (a row that the sequence uses), columns and ids are clamped.
+  };
+  // Page ids of this lane's rows of the tile that the next fetch loads, and their
+  // slots; col: their table columns.  Rows behind the end look up its last key
+  // (a row that the sequence uses); ids are clamped, so every address lies in the
+  // pool.  Tokens, columns and slots move on by additions: a division per row
+  // and tile took as long as a quarter of the softmax.
+  int pid[NLD];
+  uint32_t slot_of[NLD], col[NLD], in_page[NLD];
+  const uint32_t P = p.P;
+  auto place = [&](uint32_t tok, uint32_t& c, uint32_t& s) __attribute__((always_inline)) {
+    c = __umulhi(tok, p.invP);
+    s = tok - c * P;
+    if (s >= P) {
+      s -= P;
+      ++c;
+    }
+  };
+  uint32_t last_col = 0, last_slot = 0;
+  if (n_tiles > 0) place((uint32_t)t_end - 1, last_col, last_slot);
+  last_col = __builtin_amdgcn_readfirstlane(last_col);
+  last_slot = __builtin_amdgcn_readfirstlane(last_slot);
+#pragma unroll
+  for (int i = 0; i < NLD; ++i) place((uint32_t)(t_begin + 32 * kg + srow + i * (NT / CPR)), col[i], in_page[i]);
+  const uint32_t step_col = p.step_col[RB == 1], step_slot = p.step_slot[RB == 1];
   auto lookup = [&](int t) __attribute__((always_inline)) {
+    const bool tail = t_begin + 32 * t + 32 > t_end;  // uniform
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
-      const uint32_t tok = (uint32_t)min(t_begin + 32 * t + srow + i * (NT / CPR), t_end - 1);
-      uint32_t col;
-      if (p.log2P >= 0) {
-        col = tok >> p.log2P;
-      } else {  // floor(tok / P): the high product is it or one less
-        col = __umulhi(tok, p.invP);
-        col += tok - col * (uint32_t)p.P >= (uint32_t)p.P ? 1u : 0u;
+      uint32_t c = col[i];
+      slot_of[i] = in_page[i];
+      if (tail) {
+        asm volatile("");  // a branch that is seldom taken, and not selects in every tile
+        const bool in = t_begin + 32 * t + srow + i * (NT / CPR) < t_end;
+        c = in ? c : last_col;
+        slot_of[i] = in ? slot_of[i] : last_slot;
       }
-      pslot[i] = (int)(tok - col * (uint32_t)p.P);
-      pid[i] = ptrow[min((int)col, p.max_pages - 1)];
-    }
-  };
-  // Loads tile t (whose ids are here), and the ids of tile t + KG behind it.
-  auto fetch = [&](int t) __attribute__((always_inline)) {
-    int phys[NLD], sl[NLD];
-#pragma unroll
-    for (int i = 0; i < NLD; ++i) {
-      phys[i] = min(max(pid[i], 0), p.num_pages - 1);
-      sl[i] = pslot[i];
-    }
-    lookup(t + KG);
-#pragma unroll
-    for (int i = 0; i < NLD; ++i) {
-      R0.k[i] = *reinterpret_cast<const u32x4*>(kh + (int64_t)phys[i] * p.k_sp + (int64_t)sl[i] * p.k_ss);
-      R0.v[i] = *reinterpret_cast<const u32x4*>(vh + (int64_t)phys[i] * p.v_sp + (int64_t)sl[i] * p.v_ss);
-      if constexpr (KV != KV_SAME) {
-        R0.ksc[i] = ksh[(int64_t)phys[i] * p.sc_sp];
-        R0.vsc[i] = vsh[(int64_t)phys[i] * p.sc_sp];
+      pid[i] = ptrow[c];
+      col[i] += step_col;
+      in_page[i] += step_slot;
+      if (in_page[i] >= P) {
+        in_page[i] -= P;
+        ++col[i];
       }
     }
   };
-  // A chunk as QT elements: a copy, or round_to_QT(float(x) * scale) of 8-bit
-  // codes (sc = 1 with FOLD's K: exact).
-  auto put = [&](uint16_t* dst, const u32x4& raw, float sc) __attribute__((always_inline)) {
+  // The tile that fetch_k loads next becomes the one whose ids are here, the one it
+  // loaded last that of fetch_v; tile t's ids are asked for.  They go out ahead
+  // of the rows that a caller then loads: loads return in order, so waiting for
+  // them leaves those rows in flight.
+  uint32_t k_page[NLD], k_slot[NLD], v_page[NLD], v_slot[NLD];
+  auto advance = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+      v_page[i] = k_page[i];
+      v_slot[i] = k_slot[i];
+      k_page[i] = (uint32_t)min(max(pid[i], 0), p.num_pages - 1);
+      k_slot[i] = slot_of[i];
+    }
+    lookup(t);
+  };
+  auto fetch_k = [&](Raw& R) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+      R.k[i] = *reinterpret_cast<const u32x4*>(kh + (uint64_t)k_page[i] * p.k_sp + (uint32_t)__umul24(k_slot[i], p.k_ss));
+      if constexpr (FOLD) R.ksc[i] = ksh[(uint64_t)k_page[i] * p.sc_sp];
+    }
+  };
+  auto fetch_v = [&](Raw& R, const uint32_t* page, const uint32_t* slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+      R.v[i] = *reinterpret_cast<const u32x4*>(vh + (uint64_t)page[i] * p.v_sp + (uint32_t)__umul24(slot[i], p.v_ss));
+      if constexpr (FOLD) R.vsc[i] = vsh[(uint64_t)page[i] * p.sc_sp];
+    }
+  };
+  // A chunk as QT elements: a copy, the exact values of 8-bit codes, or
+  // (scaled) round_to_QT(float(x) * sc).
+  auto put = [&](uint16_t* dst, const u32x4& raw) __attribute__((always_inline)) {
     if constexpr (KV == KV_SAME) {
       *reinterpret_cast<u32x4*>(dst) = raw;
     } else {
-      const float nb = -128.0f * sc;
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        u32x4 o;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float f[4];
-          if constexpr (KV == KV_I8) {
-            i8x4_biased(raw[2 * h2 + j], f);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = __builtin_fmaf(f[e], sc, nb);
-          } else {
-            fp8x4(raw[2 * h2 + j], f);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = f[e] * sc;
-          }
-          o[2 * j] = Pair<QT>::pack(f[0], f[1]);
-          o[2 * j + 1] = Pair<QT>::pack(f[2], f[3]);
-        }
-        *reinterpret_cast<u32x4*>(dst + 8 * h2) = o;
-      }
+      u32 o[8];
+      codes_exact<QT, KV>(raw, o);
+      *reinterpret_cast<u32x4*>(dst) = u32x4{o[0], o[1], o[2], o[3]};
+      *reinterpret_cast<u32x4*>(dst + 8) = u32x4{o[4], o[5], o[6], o[7]};
     }
   };
+  auto put_scaled = [&](uint16_t* dst, const u32x4& raw, float sc) __attribute__((always_inline)) {
+    u32 o[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float f[4];
+      if constexpr (KV == KV_I8) {
+        i8x4_biased(raw[j], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = __builtin_fmaf(f[e], sc, -128.0f * sc);
+      } else {
+        fp8x4(raw[j], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] *= sc;
+      }
+      o[2 * j] = Pair<QT>::pack(f[0], f[1]);
+      o[2 * j + 1] = Pair<QT>::pack(f[2], f[3]);
+    }
+    *reinterpret_cast<u32x4*>(dst) = u32x4{o[0], o[1], o[2], o[3]};
+    *reinterpret_cast<u32x4*>(dst + 8) = u32x4{o[4], o[5], o[6], o[7]};
+  };
   uint16_t* const tile0 = reinterpret_cast<uint16_t*>(smem) + kg * Tl::kBufs * Tl::kTile;
-  float* const ksc0 = reinterpret_cast<float*>(smem + KG * Tl::kBufs * Tl::kTile * 2) + kg * Tl::kBufs * 32;
-  auto store = [&](int t, int buf) __attribute__((always_inline)) {
+  float* const sc0 = reinterpret_cast<float*>(smem + KG * Tl::kBufs * Tl::kTile * 2) + kg * Tl::kBufs * Tl::kScaleFloats;
+  auto store_k = [&](const Raw& R, int buf) __attribute__((always_inline)) {
     if (!stages) return;
     uint16_t* const Kt = tile0 + buf * Tl::kTile;
-    uint16_t* const Vt = Kt + 32 * K_RS;
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
       const int row = srow + i * (NT / CPR);
-      // V behind the end is zero: the scores there are masked, and 0 * v stays 0
-      // whatever the last key's v holds.
-      const bool in = t_begin + 32 * t + row < t_end;
-      const u32x4 vv = {in ? R0.v[i][0] : 0u, in ? R0.v[i][1] : 0u, in ? R0.v[i][2] : 0u, in ? R0.v[i][3] : 0u};
-      put(&Kt[row * K_RS + scol * EPC], R0.k[i], FOLD ? 1.0f : R0.ksc[i]);
-      put(&Vt[row * V_RS + scol * EPC], vv, KV != KV_SAME && !in ? 0.0f : R0.vsc[i]);
+      put(&Kt[row * K_RS + scol * EPC], R.k[i]);
       if constexpr (FOLD) {
-        if (scol == 0) ksc0[buf * 32 + row] = R0.ksc[i];
+        if (scol == 0) sc0[buf * Tl::kScaleFloats + row] = R.ksc[i] * p.scale_log2;
+      }
+    }
+  };
+  auto store_v = [&](const Raw& R, int t, int buf) __attribute__((always_inline)) {
+    if (!stages) return;
+    const bool last = t_begin + 32 * t + 32 > t_end;  // uniform
+    uint16_t* const Vt = tile0 + buf * Tl::kTile + 32 * K_RS;
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+      const int row = srow + i * (NT / CPR);
+      u32x4 vv = R.v[i];
+      if constexpr (FOLD) {
+        // behind the end: a scale of 0, which the codes' finite values keep at 0
+        const float sc = !last || t_begin + 32 * t + row < t_end ? R.vsc[i] : 0.f;
+        if constexpr (FOLD_V) {
+          put(&Vt[row * V_RS + scol * EPC], vv);
+          if (scol == 0) sc0[buf * Tl::kScaleFloats + 32 + row] = sc;
+        } else {
+          put_scaled(&Vt[row * V_RS + scol * EPC], vv, sc);
+        }
+      } else {
+        if (last) {
+          asm volatile("");  // a branch
+          // behind the end: zeros; the scores there are masked, and 0 * v stays 0
+          // whatever the last key's v holds
+          const bool in = t_begin + 32 * t + row < t_end;
+          vv = u32x4{in ? vv[0] : 0u, in ? vv[1] : 0u, in ? vv[2] : 0u, in ? vv[3] : 0u};
+        }
+        put(&Vt[row * V_RS + scol * EPC], vv);
       }
     }
   };
@@ -246,15 +357,14 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
   float m_run = -INFINITY;  // log2 units
   float l_run = 0.f;
-  const float c = p.scale_log2;
   const int tr_c = (lane & 15) >> 2, tr_j = lane & 3, tr_G = lane >> 4;
   const int tr_row = 4 * (tr_G >> 1) + tr_c;
   const int tr_col = 16 * (tr_G & 1) + 4 * tr_j;
 
-  auto compute = [&](int t, int buf) __attribute__((always_inline)) {
+  // S^T of the keys in K buffer `buf` (in log2 units for 8-bit caches, whose
+  // scales it applies): row li over keys (r & 3) + 4 g + 8 (r >> 2).
+  auto qk = [&](f32x16& s, int buf) __attribute__((always_inline)) {
     const uint16_t* const Kt = tile0 + buf * Tl::kTile;
-    const uint16_t* const Vt = Kt + 32 * K_RS;
-    f32x16 s;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
@@ -262,23 +372,28 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
       const u32x4 a = *reinterpret_cast<const u32x4*>(&Kt[li * K_RS + 16 * ks + 8 * g]);
       s = Mfma<QT>::mma(a, qf[ks], s);
     }
-    // Row li over keys kb + (r & 3) + 4 g + 8 (r >> 2).
-    const int kb = t_begin + 32 * t;
-    f32x4 ck[4];
+  };
+  auto scale_s = [&](f32x16& s, int buf) __attribute__((always_inline)) {
     if constexpr (FOLD) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ck[j] = *reinterpret_cast<const f32x4*>(&ksc0[buf * 32 + 4 * g + 8 * j]) * c;
-    }
-    float mx = -INFINITY;
-    const bool masked = kb + 32 > all_end;  // uniform
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 ck = *reinterpret_cast<const f32x4*>(&sc0[buf * Tl::kScaleFloats + 4 * g + 8 * j]);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float x = s[r] * (FOLD ? ck[r >> 2][r & 3] : c);
-      if (masked) x = kb + (r & 3) + 4 * g + 8 * (r >> 2) < my_end ? x : -INFINITY;
-      s[r] = x;
-      mx = fmaxf(mx, x);
+        for (int e = 0; e < 4; ++e) s[4 * j + e] *= ck[e];
+      }
     }
-    mx = xor32<OpMax>(mx);
+  };
+  const float c = FOLD ? 1.f : p.scale_log2;
+  auto mask = [&](f32x16& s, int t) __attribute__((always_inline)) {
+    const int kb = t_begin + 32 * t;
+    if (kb + 32 > all_end) {  // uniform
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = kb + (r & 3) + 4 * g + 8 * (r >> 2) < my_end ? s[r] : -INFINITY;
+    }
+  };
+  // Moves the running maximum to one of mx, a lane's largest score.
+  auto raise = [&](float mx) __attribute__((always_inline)) {
+    mx = xor32<OpMax>(mx) * c;
     if (__any(mx > m_run + kSharedLazy)) {
       const bool grow = mx > m_run + kSharedLazy;
       const float alpha = grow ? fast_exp2(m_run - mx) : 1.f;
@@ -289,66 +404,158 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
     }
-    // A row that has seen no key yet keeps m = -inf; its scores are -inf too,
-    // and 2^(-inf - 0) = 0.
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
-    u32x4 pf[2], pl[2];
+  };
+  auto largest = [&](const f32x16& s) __attribute__((always_inline)) {
+    float mx = max3(s[0], s[1], s[2]);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int r = 3; r < 15; r += 2) mx = max3(mx, s[r], s[r + 1]);
+    return fmaxf(mx, s[15]);
+  };
+  u32x4 pf[2], pl[2];
+  // Scores 2 j and 2 j + 1 as P = 2^(s - m), times v_scale where V is staged as
+  // codes.  m_use: a row that has seen no key yet keeps m = -inf; its scores are
+  // -inf too, and 2^(-inf - 0) = 0.
+  float m_use = 0.f;
+  f32x4 cv[4];
+  auto load_cv = [&](int buf) __attribute__((always_inline)) {
+    m_use = m_run == -INFINITY ? 0.f : m_run;
+    if constexpr (FOLD_V) {
 #pragma unroll
-      for (int e2 = 0; e2 < 4; ++e2) {
-        const float x0 = fast_exp2(s[8 * u + 2 * e2] - m_use);
-        const float x1 = fast_exp2(s[8 * u + 2 * e2 + 1] - m_use);
-        l_run += x0 + x1;
-        const u32 hp = Pair<QT>::pack(x0, x1);
-        pf[u][e2] = hp;
-        if constexpr (SPLIT_P) pl[u][e2] = Pair<QT>::pack(x0 - Pair<QT>::lo(hp), x1 - Pair<QT>::hi(hp));
-      }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int vrow = 16 * u + tr_row;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const uint16_t* vp = &Vt[vrow * V_RS + 32 * db + tr_col];
-        const u32x2 lo = lds_read_tr16(vp);
-        const u32x2 hi = lds_read_tr16(vp + 8 * V_RS);
-        const u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
-        acc[db] = Mfma<QT>::mma(a, pf[u], acc[db]);
-        if constexpr (SPLIT_P) acc[db] = Mfma<QT>::mma(a, pl[u], acc[db]);
-      }
+      for (int j = 0; j < 4; ++j) cv[j] = *reinterpret_cast<const f32x4*>(&sc0[buf * Tl::kScaleFloats + 32 + 4 * g + 8 * j]);
     }
+  };
+  auto piece = [&](const f32x16& s, int j) __attribute__((always_inline)) {
+    float x0 = fast_exp2(FOLD ? s[2 * j] - m_use : __builtin_fmaf(s[2 * j], c, -m_use));
+    float x1 = fast_exp2(FOLD ? s[2 * j + 1] - m_use : __builtin_fmaf(s[2 * j + 1], c, -m_use));
+    l_run += x0 + x1;
+    if constexpr (FOLD_V) {
+      x0 *= cv[j >> 1][2 * (j & 1)];
+      x1 *= cv[j >> 1][2 * (j & 1) + 1];
+    }
+    const u32 hp = Pair<QT>::pack(x0, x1);
+    pf[j >> 2][j & 3] = hp;
+    if constexpr (SPLIT_P) pl[j >> 2][j & 3] = Pair<QT>::pack(x0 - Pair<QT>::lo(hp), x1 - Pair<QT>::hi(hp));
+  };
+  // O^T += V^T P^T: entry e is keys 16 u .. + 15 of the tile (u = e / DB), dims 32 db ..
+  // + 31 (db = e % DB).
+  auto read_v = [&](int buf, int e) __attribute__((always_inline)) {
+    const uint16_t* vp = tile0 + buf * Tl::kTile + 32 * K_RS + (16 * (e / DB) + tr_row) * V_RS + 32 * (e % DB) + tr_col;
+    const u32x2 lo = lds_read_tr16(vp);
+    const u32x2 hi = lds_read_tr16(vp + 8 * V_RS);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto pv = [&](const u32x4& a, int e) __attribute__((always_inline)) {
+    acc[e % DB] = Mfma<QT>::mma(a, pf[e / DB], acc[e % DB]);
+    if constexpr (SPLIT_P) acc[e % DB] = Mfma<QT>::mma(a, pl[e / DB], acc[e % DB]);
   };
 
   if constexpr (RB == 1) {
     // Each wave has its own tiles: no workgroup barrier.
+    Raw R;
+    f32x16 s;
     if (kg < n_tiles) {
       lookup(kg);
-      fetch(kg);
+      advance(kg + KG);
+      fetch_k(R);
+      fetch_v(R, k_page, k_slot);
     }
     for (int t = kg; t < n_tiles; t += KG) {
-      store(t, 0);
-      if (t + KG < n_tiles) fetch(t + KG);
+      store_k(R, 0);
+      store_v(R, t, 0);
+      if (t + KG < n_tiles) {
+        advance(t + 2 * KG);
+        fetch_k(R);
+        fetch_v(R, k_page, k_slot);
+      }
       wave_lds_fence();
-      compute(t, 0);
+      qk(s, 0);
+      scale_s(s, 0);
+      mask(s, t);
+      raise(largest(s));
+      load_cv(0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) piece(s, j);
+#pragma unroll
+      for (int e = 0; e < 2 * DB; ++e) pv(read_v(0, e), e);
       wave_lds_fence();
     }
   } else {
-    // The same number of rounds for all key groups (the barriers): a round behind
-    // the end stages zeros of the last key's page and masks them all.
+    // Round i: S = K Q^T of tile i + 1 beside the exponentials of tile i, then O += V P
+    // of tile i beside the maximum of tile i + 1.  K(i + 1) and V(i) lie in LDS, K(i +
+    // 2) and V(i + 1) in registers (loaded a round ago, stored at this one's end),
+    // and K(i + 3) and V(i + 2) are loaded.  One barrier a round: behind it every wave is
+    // done with round i - 1, whose buffers the round's stores take.  All key groups
+    // run the same number of rounds; tiles behind the end stage the last key, and
+    // their scores are masked.
     const int rounds = (n_tiles + KG - 1) / KG;
     if (rounds > 0) {
+      Raw Ra, Rb;
+      f32x16 sa, sb;
       lookup(kg);
-      fetch(kg);
-      store(kg, 0);
-    }
-    for (int i = 0; i < rounds; ++i) {
-      const int t = kg + i * KG;
-      if (i + 1 < rounds) fetch(t + KG);
-      // Tile i is here, and every wave is done with tile i - 1, whose buffer the
-      // next store takes.
+      advance(kg + KG);
+      fetch_k(Ra);
+      fetch_v(Ra, k_page, k_slot);
+      advance(kg + 2 * KG);
+      fetch_k(Rb);
+      fetch_v(Rb, k_page, k_slot);
+      advance(kg + 3 * KG);
+      store_k(Ra, 0);
+      store_v(Ra, kg, 0);
+      store_k(Rb, 1);
+      fetch_k(Rb);
       __syncthreads();
-      compute(t, i & 1);
-      if (i + 1 < rounds) store(t + KG, (i + 1) & 1);
+      qk(sa, 0);
+      scale_s(sa, 0);
+      mask(sa, kg);
+      raise(largest(sa));
+      auto round = [&](int i, f32x16& s, f32x16& s2, const Raw& X, Raw& Y) __attribute__((always_inline)) {
+        const int t = kg + i * KG;
+        const int now = i & 1, next = now ^ 1;
+        advance(t + 4 * KG);
+        fetch_v(Y, v_page, v_slot);
+        fetch_k(Y);
+        __syncthreads();
+        load_cv(now);
+        // A part of the softmax in the shadow of each MFMA; LDS reads run LOOK entries
+        // ahead of theirs.  sched_barrier keeps the steps apart: left to itself the
+        // compiler lines the MFMAs up behind the exponentials.
+        constexpr int LOOK = 3;
+        const uint16_t* const Kn = tile0 + next * Tl::kTile + li * K_RS + 8 * g;
+        u32x4 ka[KS], va[2 * DB];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s2[r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < LOOK; ++k) ka[k] = *reinterpret_cast<const u32x4*>(Kn + 16 * k);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          s2 = Mfma<QT>::mma(ka[k], qf[k], s2);
+          if (k + LOOK < KS) ka[k + LOOK] = *reinterpret_cast<const u32x4*>(Kn + 16 * (k + LOOK));
+          else va[k + LOOK - KS] = read_v(now, k + LOOK - KS);
+#pragma unroll
+          for (int j = 8 * k / KS; j < 8 * (k + 1) / KS; ++j) piece(s, j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        float mx = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2 * DB; ++e) {
+          pv(va[e], e);
+          if (e + LOOK < 2 * DB) va[e + LOOK] = read_v(now, e + LOOK);
+          if (e == DB / 2 - 1) {
+            scale_s(s2, next);
+            mask(s2, t + KG);
+          }
+          if (e == DB) mx = largest(s2);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        raise(mx);
+        store_k(X, now);
+        store_v(X, t + KG, next);
+      };
+      for (int i = 0; i < rounds; i += 2) {
+        round(i, sa, sb, Rb, Ra);
+        if (i + 1 < rounds) round(i + 1, sb, sa, Ra, Rb);  // uniform
+      }
     }
   }
 
@@ -428,7 +635,7 @@ void decode_shared_kernel(const SharedParams p) {
                              : SharedTile<QT, KV, D, 1>::kBytes;
   __shared__ __attribute__((aligned(16))) uint8_t smem[kBytes];
   const int S = p.prefix_split + p.split;
-  const int cap = p.max_pages * p.P;
+  const int cap = p.max_pages * p.P;  // all token places are below it: columns below max_pages
   if ((int)blockIdx.x < p.prefix_blocks) {
     // Row tiles of the same keys run 8 ids apart, on one XCD, and meet in its L2.
     const int step = 8 * p.tiles;
@@ -469,7 +676,7 @@ void decode_shared_kernel(const SharedParams p) {
 }
 
 // Joins a row's S partials, one wave per row: lane s has those of slots s and s +
-// 64.  Slots of weight 0 (no keys) are not read.
+// 64.  Slots of weight 0 (no keys) do not count.
 constexpr int kJoinRows = 4;
 template <typename QT, int D>
 __global__ __launch_bounds__(64 * kJoinRows) void shared_join_kernel(const SharedParams p) {
@@ -505,11 +712,19 @@ __global__ __launch_bounds__(64 * kJoinRows) void shared_join_kernel(const Share
 #pragma unroll
   for (int e = 0; e < E; ++e) a[e] = 0.f;
   const float* acc = p.ws_acc + row * S * D + E * lane;
-  for (int s = 0; s < S; ++s) {
-    const float w = __shfl(s < 64 ? f[0] : f[1], s & 63);
-    if (w != 0.f) {  // uniform
+  // Eight slots' loads in flight; those of weight 0 may never have been written.
+  for (int s0 = 0; s0 < S; s0 += 8) {
+    float x[8][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) a[e] = __builtin_fmaf(acc[(int64_t)s * D + e], w, a[e]);
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][e] = acc[(int64_t)min(s0 + i, S - 1) * D + e];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i;
+      const float w = __shfl(s < 64 ? f[0] : f[1], s & 63);  // 0 for s >= S
+#pragma unroll
+      for (int e = 0; e < E; ++e) a[e] = __builtin_fmaf(w != 0.f ? x[i][e] : 0.f, w, a[e]);
     }
   }
   const int64_t bt = row / p.H;
@@ -533,7 +748,6 @@ void launch_shared_d(const fat::SharedParams& prm, int rb, unsigned blocks, hipS
   const dim3 block(64 * fat::kSharedWaves);
   switch (rb) {
     case 4: hipLaunchKernelGGL((fat::decode_shared_kernel<QT, KV, D, 4>), dim3(blocks), block, 0, stream, prm); break;
-    case 2: hipLaunchKernelGGL((fat::decode_shared_kernel<QT, KV, D, 2>), dim3(blocks), block, 0, stream, prm); break;
     default: hipLaunchKernelGGL((fat::decode_shared_kernel<QT, KV, D, 1>), dim3(blocks), block, 0, stream, prm); break;
   }
 }
@@ -598,6 +812,10 @@ extern "C" int fat_paged_decode_shared(const fat_shared_args* a, void* stream_pt
                         a->prefix_chunk, a->chunk, a->q_len);
     return FAT_E_INVALID;
   }
+  if (a->row_blocks != 0 && a->row_blocks != 1 && a->row_blocks != 4) {
+    fat_host::set_error("fat_paged_decode_shared: row_blocks must be 0 (by the rows), 1 or 4, got %d", a->row_blocks);
+    return FAT_E_INVALID;
+  }
   if ((int64_t)a->prefix_split * a->prefix_chunk > 0x7fffffffLL || (int64_t)a->split * a->chunk > 0x7fffffffLL) {
     fat_host::set_error("fat_paged_decode_shared: splits times chunk overflow int32 positions");
     return FAT_E_INVALID;
@@ -629,6 +847,18 @@ extern "C" int fat_paged_decode_shared(const fat_shared_args* a, void* stream_pt
     fat_host::set_error("fat_paged_decode_shared: q, K, V and workspace pointers and row strides must be 16-byte aligned");
     return FAT_E_INVALID;
   }
+  // K/V offsets are products of 32-bit (page) and 24-bit (slot) factors; a page's
+  // rows lie within 4 GiB of its start.
+  auto fits = [&](int64_t sp, int64_t ss) {
+    return sp >= 0 && ss >= 0 && eb * sp < (1LL << 32) && eb * ss < (1LL << 24) && a->page_size < (1 << 24) &&
+           eb * ss * (int64_t)a->page_size < (1LL << 32);
+  };
+  if (!fits(a->k_stride_page, a->k_stride_slot) || !fits(a->v_stride_page, a->v_stride_slot) ||
+      a->scale_stride_page < 0 || a->scale_stride_page >= (1LL << 32)) {
+    fat_host::set_error("fat_paged_decode_shared: K/V strides must be non-negative, pages below 4 GiB "
+                        "and slots below 16 MiB apart");
+    return FAT_E_UNSUPPORTED;
+  }
   const int S = a->prefix_split + a->split;
   const size_t need = fat_paged_decode_shared_workspace_bytes(a->batch * T, a->num_heads, a->head_dim, S);
   if (a->workspace_bytes < (int64_t)need) {
@@ -655,13 +885,13 @@ extern "C" int fat_paged_decode_shared(const fat_shared_args* a, void* stream_pt
   prm.o_sb = a->out_stride_b;
   prm.o_st = T > 1 ? a->out_stride_t : 0;
   prm.o_sh = a->out_stride_h;
-  prm.k_sp = eb * a->k_stride_page;
-  prm.k_ss = eb * a->k_stride_slot;
+  prm.k_sp = (uint32_t)(eb * a->k_stride_page);
+  prm.k_ss = (uint32_t)(eb * a->k_stride_slot);
   prm.k_sh = eb * a->k_stride_head;
-  prm.v_sp = eb * a->v_stride_page;
-  prm.v_ss = eb * a->v_stride_slot;
+  prm.v_sp = (uint32_t)(eb * a->v_stride_page);
+  prm.v_ss = (uint32_t)(eb * a->v_stride_slot);
   prm.v_sh = eb * a->v_stride_head;
-  prm.sc_sp = a->scale_stride_page;
+  prm.sc_sp = (uint32_t)a->scale_stride_page;
   prm.sc_sh = a->scale_stride_head;
   prm.pt_sb = a->page_table_stride;
   prm.B = a->batch;
@@ -671,19 +901,24 @@ extern "C" int fat_paged_decode_shared(const fat_shared_args* a, void* stream_pt
   prm.Hkv = a->num_kv_heads;
   prm.group = a->num_heads / a->num_kv_heads;
   prm.P = a->page_size;
-  prm.log2P = -1;
-  for (int l = 0; l < 31; ++l)
-    if (a->page_size == (1 << l)) prm.log2P = l;
-  prm.invP = a->page_size > 1 ? (uint32_t)((uint64_t(1) << 32) / (uint32_t)a->page_size) : 0;
+  prm.invP = a->page_size > 1 ? (uint32_t)((uint64_t(1) << 32) / (uint32_t)a->page_size) : 0xffffffffu;
   prm.num_pages = a->num_pages;
   prm.max_pages = a->max_pages;
-  prm.scale_log2 = a->softmax_scale * fat::kLog2e;
+  const float scale = a->softmax_scale;
+  prm.scale_log2 = (scale == 0.f ? 1.f : scale < 0.f ? -scale : scale) * fat::kLog2e;
+  prm.q_and = scale == 0.f ? 0u : ~0u;
+  prm.q_xor = scale < 0.f ? 0x80008000u : 0u;
   prm.prefix_split = a->prefix_split;
   prm.prefix_chunk = a->prefix_chunk;
   prm.split = a->split;
   prm.chunk = a->chunk;
   const int64_t rows = (int64_t)std::min(a->max_group, a->batch) * T * prm.group;
-  const int rb = 1;
+  const int rb = a->row_blocks ? a->row_blocks : rows > 32 ? 4 : 1;
+  for (int own = 0; own < 2; ++own) {
+    const uint32_t step = 32 * (own ? fat::kSharedWaves : fat::kSharedWaves / rb);
+    prm.step_col[own] = step / (uint32_t)a->page_size;
+    prm.step_slot[own] = step % (uint32_t)a->page_size;
+  }
   const int64_t tiles = (rows + 32 * rb - 1) / (32 * rb);
   const int64_t units = (int64_t)a->groups * a->prefix_split * a->num_kv_heads;
   const int64_t own_tiles = (T * prm.group + 31) / 32;

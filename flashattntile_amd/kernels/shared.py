@@ -23,7 +23,8 @@ __all__ = ["paged_decode_attention_shared", "paged_decode_shared_launch", "share
 
 # Partials of a launch: prefix_split chunks of prefix_chunk keys of a group's
 # prefix, split chunks of chunk keys of a sequence's own; None: shared_splits.
-_CONFIG_KEYS = ("prefix_split", "split")
+# row_blocks: rows of a workgroup on a prefix, in 32s (1 or 4; None: by the rows).
+_CONFIG_KEYS = ("prefix_split", "split", "row_blocks")
 
 
 def _check_inputs(q, cache: PagedKVCache, cu_groups, prefix_lens, scales) -> None:
@@ -105,6 +106,9 @@ def _takes(q, cache: PagedKVCache) -> bool:
     if cache.capacity > 2 ** 31 - 4097:
         return False
     eb = k.element_size()
+    if cache.page_size >= 2 ** 24 or any(eb * t.stride(0) >= 2 ** 32 or eb * t.stride(1) >= 2 ** 24 or
+                                         eb * t.stride(1) * cache.page_size >= 2 ** 32 for t in (k, v)):
+        return False
     words = [k.data_ptr(), v.data_ptr(), q.data_ptr()]
     words += [eb * s for t in (k, v) for s in t.stride()[:3]]
     return all(x % 16 == 0 for x in words)
@@ -155,6 +159,7 @@ def _launch(a, q, cfg: dict, max_group: int, workspace=None) -> None:
     a.max_group = max_group
     a.prefix_split, a.prefix_chunk = cfg["prefix_split"], cfg["prefix_chunk"]
     a.split, a.chunk = cfg["split"], cfg["chunk"]
+    a.row_blocks = cfg.get("row_blocks", 0)
     _hip.shared_with_args(a, workspace, _hip.current_stream_handle(q.device))
 
 
@@ -195,11 +200,16 @@ def _resolve(config, q, cache, groups: int, max_prefix: int, max_own: int, max_g
     if unknown:
         raise ValueError(f"unknown shared decode config keys: {sorted(unknown)}")
     given = {k: v for k, v in config.items() if v is not None}
+    row_blocks = given.pop("row_blocks", 0)
+    if row_blocks not in (0, 1, 4):
+        raise ValueError(f"row_blocks must be None, 1 or 4, got {row_blocks}")
     for k, v in given.items():
         if not isinstance(v, int) or isinstance(v, bool) or not 1 <= v <= 64:
             raise ValueError(f"{k} must be an integer in [1, 64], got {v}")
-    return _chunks(given.get("prefix_split", cfg["prefix_split"]), given.get("split", cfg["split"]), max_prefix,
-                   max_own)
+    cfg = _chunks(given.get("prefix_split", cfg["prefix_split"]), given.get("split", cfg["split"]), max_prefix,
+                  max_own)
+    cfg["row_blocks"] = row_blocks
+    return cfg
 
 
 def paged_decode_attention_shared(

@@ -519,11 +519,12 @@ int fat_append_kv(const fat_append_args* args, void* stream);
  * are the same, and are read through the table row of the group's first
  * sequence.  seq_lens counts all keys, the shared ones among them; prefix_lens[g]
  * <= seq_lens[b] - q_len + 1.  A prefix of 0 keys and groups of one or no
- * sequence are valid.  Layouts, q_len and 8-bit caches as for fat_paged_decode;
+ * sequence are valid.  Layouts and q_len as for fat_paged_decode;
  * fp16/bf16 queries, head_dim 64 or 128, any page size (FAT_E_UNSUPPORTED
  * otherwise), 16-byte aligned q, K, V and workspace rows.  Lengths, offsets and
  * page ids are clamped on the device: bad ones give wrong answers, never an
- * access out of bounds.
+ * access out of bounds.  8-bit caches: exact codes, k_scale on the fp32 scores;
+ * v_scale on P with bf16 queries, V as round_to_fp16(x * v_scale) with fp16 ones.
  * The shared keys are cut into prefix_split partials of prefix_chunk keys, a
  * sequence's own into split partials of chunk keys (multiples of 32; the last
  * takes any keys beyond), joined by log-sum-exp through `workspace`, which holds
@@ -564,6 +565,8 @@ typedef struct fat_shared_args {
   int32_t kv_dtype;
   int32_t prefix_split, prefix_chunk;
   int32_t split, chunk;
+  int32_t row_blocks; /* rows of a workgroup on a prefix / 32: 1 or 4; 0: by
+                         the largest group's rows */
   float softmax_scale;
 } fat_shared_args;
 

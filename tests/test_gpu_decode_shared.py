@@ -6,9 +6,8 @@ second product as fp16 (half a step, 2^-11 of each p; a p in fp16's subnormals i
 off by 2^-25 of the largest at most, n keys of them) or as two bf16 (2^-16), so
 that a weighted mean of v moves by that share of max |v|; fp32 scores of up to 64
 (log2 units, 2^-24 each, and the sums) move p by less than 2^-16; and the output's
-own rounding is half a step.  8-bit caches are compared on the values the decode
-contract gives them: K and V rounded to bf16 after scaling, or, with fp16 queries,
-exact K times its scale and V rounded to fp16.
+own rounding is half a step.  8-bit caches are compared on code times scale, with
+fp16 queries on V rounded to fp16 after that.
 """
 
 from __future__ import annotations
@@ -83,18 +82,16 @@ def _setup(groups, P, hkv, d, dtype, tokens=1, heads=8, kv="same", seed=0, spare
 
 
 def _values(cache, scales, dtype):
-    """K and V pages in 64 bits, as the decode contract has 8-bit ones."""
+    """K and V pages in 64 bits."""
     out = []
     for name, x in (("k", cache.k_cache), ("v", cache.v_cache)):
         if scales is None:
             out.append(x.double().cpu())
             continue
-        y = x.float().cpu() * scales[name].float().cpu()[:, None, :, None]
-        if name == "k" and dtype == torch.float16:
-            y = x.double().cpu() * scales[name].double().cpu()[:, None, :, None]
-        else:
-            y = y.to(dtype)
-        out.append(y.double())
+        y = x.double().cpu() * scales[name].double().cpu()[:, None, :, None]
+        if name == "v" and dtype == torch.float16:
+            y = (x.float().cpu() * scales[name].cpu()[:, None, :, None]).half().double()
+        out.append(y)
     return out
 
 
@@ -169,7 +166,8 @@ def test_rows_of_a_group_and_splits(dtype, kv, sequences):
     case = _setup(groups, 16, 2, 128, DTYPES[dtype], 0, 8, kv, seed=sequences)
     ref = _reference(case["q"], case["cache"], case["scales"])
     for config in (None, {"prefix_split": 1, "split": 1}, {"prefix_split": 5}, {"prefix_split": 64, "split": 64},
-                   {"split": 3}):
+                   {"split": 3}, {"row_blocks": 1}, {"row_blocks": 4},
+                   {"row_blocks": 1, "prefix_split": 2}, {"row_blocks": 4, "prefix_split": 3}):
         print(f"sequences {sequences} {dtype} {kv} {config}", flush=True)
         out = _run(case, config=config)
         _check(out, *ref, f"{sequences} {dtype} {kv} {config}")
@@ -305,6 +303,7 @@ def test_refusals():
     refused("unknown shared decode config", config={"split_k": 2})
     refused("prefix_split must be", config={"prefix_split": 65})
     refused("split must be", config={"split": 0})
+    refused("row_blocks must be", config={"row_blocks": 3})
     # what lies on the device
     refused("start at 0", cu=_ints([1, 2, 3]))
     refused("end at the batch size", cu=_ints([0, 1, 2]))
