@@ -21,7 +21,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libfat_hip.so"
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 # enum fat_dtype
 DT_F16 = 0
@@ -469,7 +469,6 @@ class CheckArgs(ctypes.Structure):
         ("values", _c_vp),
         ("count", _c_i64),
         ("ids", _c_vp * 3),
-        ("scratch", _c_vp),
         ("num_pages", _c_i32),
         ("tokens", _c_i32),
     ]
@@ -596,7 +595,7 @@ class Check:
 
     def begin(self, kind: int, batch: int, stream: int, cu_q: torch.Tensor | None, cu_k: torch.Tensor | None,
               seq_lens: torch.Tensor | None, page_table: torch.Tensor | None, page_size: int, ids=(),
-              scratch: torch.Tensor | None = None, num_pages: int = 0, tokens: int = 1) -> None:
+              num_pages: int = 0, tokens: int = 1) -> None:
         if self._pending:
             torch.cuda.synchronize(self._device)
         a = self._args
@@ -606,7 +605,6 @@ class Check:
             a.count = ids[0].numel()
             for i, t in enumerate(ids):
                 a.ids[i] = t.data_ptr()
-            a.scratch = _ptr(scratch)
             a.num_pages = num_pages
             a.tokens = tokens
         a.cu_q = None if cu_q is None else cu_q.data_ptr()
@@ -673,17 +671,15 @@ def float_range(values: torch.Tensor) -> tuple[float, float]:
 def check_begin(kind: int, stream: int, device: torch.device, cu_q: torch.Tensor | None = None,
                 cu_k: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None,
                 page_table: torch.Tensor | None = None, page_size: int = 0, ids=(),
-                scratch: torch.Tensor | None = None, num_pages: int = 0, tokens: int = 1) -> Check:
+                num_pages: int = 0, tokens: int = 1) -> Check:
     """Begin a check on ``stream``: ``cu_q`` / ``cu_k`` int32 [B + 1],
     ``seq_lens`` int32 [B] (contiguous), ``page_table`` int32 [B, M > 0] with
     a unit column stride, B > 0, on one ROCm device; ``ids``: the int32 lists
-    (contiguous, of one length) of a check of page operations, ``scratch`` its
-    int32 scratch memory; of a shared-prefix decode the prefixes, with its
-    ``tokens`` per sequence."""
+    (contiguous, of one length) of a check of page operations, or the prefixes of
+    a shared-prefix decode, with its ``tokens`` per sequence."""
     check = _thread_check(device)
     batch = seq_lens.shape[0] if seq_lens is not None else cu_q.shape[0] - 1 if cu_q is not None else 0
-    check.begin(kind, batch, stream, cu_q, cu_k, seq_lens, page_table, page_size, ids, scratch, num_pages,
-                tokens)
+    check.begin(kind, batch, stream, cu_q, cu_k, seq_lens, page_table, page_size, ids, num_pages, tokens)
     return check
 
 

@@ -26,15 +26,18 @@ struct Plane {
   uint32_t inner;           // rows per outer step
   uint32_t vpr;             // vectors per row
   uint32_t vpp;             // vectors per page
-  uint32_t ppw;             // pages per workgroup step (vpp small), or 1
-  uint32_t spp;             // workgroup steps per page (vpp large), or 1
+  uint32_t inv;             // floor(2^32 / vpp) (vpp > 1)
+  uint32_t cpp;             // chunks of 1 KiB per page; 0: its pages aren't runs of whole ones
   int32_t log2v;            // log2 of the vector's bytes
 };
 
 constexpr int kMaxPlanes = 6;
 constexpr int kCopyThreads = 256;
-constexpr int kCopyUnroll = 8;  // vectors per thread and step: 32 KiB of 16-byte vectors
-constexpr uint32_t kCopyStep = kCopyThreads * kCopyUnroll;
+constexpr int kChunk = 1024;     // bytes: 16 per lane of a wave
+constexpr int kWaveChunks = 8;   // per wave and step
+constexpr int kStepChunks = kCopyThreads / 64 * kWaveChunks;
+constexpr int kVectors = 2;      // per thread and step
+constexpr int kStepVectors = kVectors * kCopyThreads;
 
 struct Planes {
   Plane p[kMaxPlanes];
@@ -42,79 +45,106 @@ struct Planes {
   int32_t num_pages;
 };
 
-__device__ __forceinline__ int64_t plane_offset(const Plane& pl, uint32_t v) {
-  if (v < pl.vpr) return (int64_t)v << pl.log2v;  // the first row, or a page that is one row
-  const uint32_t r = v / pl.vpr;
-  const uint32_t o = r / pl.inner;
-  return (int64_t)o * pl.outer_stride + (int64_t)(r - o * pl.inner) * pl.inner_stride +
-         ((int64_t)(v - r * pl.vpr) << pl.log2v);
+__device__ __forceinline__ int64_t plane_steps(const Plane& pl, int64_t count) {
+  return pl.cpp ? (count * pl.cpp + kStepChunks - 1) / kStepChunks : (count * pl.vpp + kStepVectors - 1) / kStepVectors;
 }
 
-template <typename V>
-__device__ __forceinline__ void copy_vec(const uint8_t* src, uint8_t* dst) {
-  *reinterpret_cast<V*>(dst) = *reinterpret_cast<const V*>(src);
+// Quotient and remainder of uniform numbers.
+__device__ __forceinline__ int64_t divide(int64_t x, uint32_t by, uint32_t& rest) {
+  const int64_t q = x <= 0xffffffffll ? (int64_t)((uint32_t)x / by) : x / by;
+  rest = (uint32_t)(x - q * by);
+  return q;
 }
 
-// The pages of one workgroup step of a plane: pair(i, src, dst) gives the ids
-// of pair i < count and whether it is to be copied.
+// Pages that are runs of 1 KiB chunks (all but slices of a pool, and scales):
+// 32 chunks of them, 8 per wave.  A chunk has one pair of ids, so its addresses
+// are scalar, and a lane holds nothing but its 16 bytes of each chunk: all of a
+// wave's loads are in flight before its first store, at full occupancy.
+template <typename Pair>
+__device__ __forceinline__ void copy_chunks(const Plane& pl, int64_t step, int64_t count, Pair pair) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lane = (threadIdx.x & 63) * 16;
+  uint32_t c;
+  int64_t i = divide(step * kStepChunks + wave * kWaveChunks, pl.cpp, c);
+  u32x4 x[kWaveChunks];
+  uint8_t* to[kWaveChunks];
+  int s = 0, d = 0;
+  bool on = i < count && pair(i, s, d);
+#pragma unroll
+  for (int u = 0; u < kWaveChunks; ++u) {
+    to[u] = nullptr;
+    if (on) {
+      x[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(pl.base + (int64_t)s * pl.page + (int64_t)c * kChunk + lane));
+      to[u] = pl.base + (int64_t)d * pl.page + (int64_t)c * kChunk;
+    }
+    if (++c == pl.cpp) {
+      c = 0;
+      ++i;
+      on = i < count && pair(i, s, d);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kWaveChunks; ++u)
+    if (to[u]) *reinterpret_cast<u32x4*>(to[u] + lane) = x[u];
+}
+
+// Any other plane: 512 vectors of its pages (more per thread spilled).
 template <typename V, typename Pair>
+__device__ __forceinline__ void copy_vectors(const Plane& pl, int64_t step, int64_t count, Pair pair) {
+  uint32_t rest;
+  const int64_t i0 = divide(step * kStepVectors, pl.vpp, rest);
+  V x[kVectors];
+  uint8_t* to[kVectors];
+#pragma unroll
+  for (int u = 0; u < kVectors; ++u) {
+    uint32_t v = rest + threadIdx.x + u * kCopyThreads;
+    uint32_t k = pl.vpp > 1 ? __umulhi(v, pl.inv) : v;  // v / vpp, or one less
+    v -= k * pl.vpp;
+    if (v >= pl.vpp) {
+      v -= pl.vpp;
+      ++k;
+    }
+    int s, d;
+    to[u] = nullptr;
+    if (i0 + k < count && pair(i0 + k, s, d)) {
+      const uint32_t r = v / pl.vpr;
+      const uint32_t o = r / pl.inner;
+      const int64_t off = (int64_t)o * pl.outer_stride + (int64_t)(r - o * pl.inner) * pl.inner_stride +
+                          (int64_t)(v - r * pl.vpr) * (int64_t)sizeof(V);
+      x[u] = *reinterpret_cast<const V*>(pl.base + (int64_t)s * pl.page + off);
+      to[u] = pl.base + (int64_t)d * pl.page + off;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kVectors; ++u)
+    if (to[u]) *reinterpret_cast<V*>(to[u]) = x[u];
+}
+
+// pair(i, src, dst) gives the ids of pair i and whether it is to be copied.
+template <typename Pair>
 __device__ __forceinline__ void copy_step(const Plane& pl, int64_t step, int64_t count, Pair pair) {
-  if (pl.ppw == 1) {
-    // 32 KiB of one page: its ids are the same for the whole workgroup.
-    const int64_t i = step / pl.spp;
-    const uint32_t v0 = (uint32_t)(step - i * pl.spp) * kCopyStep;
-    int src, dst;
-    if (!pair(i, src, dst)) return;
-    const uint8_t* s = pl.base + (int64_t)src * pl.page;
-    uint8_t* d = pl.base + (int64_t)dst * pl.page;
-    V x[kCopyUnroll];
-    int64_t off[kCopyUnroll];
-#pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u) {
-      const uint32_t v = v0 + u * kCopyThreads + threadIdx.x;
-      off[u] = plane_offset(pl, v);
-      if (v < pl.vpp) x[u] = *reinterpret_cast<const V*>(s + off[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u) {
-      const uint32_t v = v0 + u * kCopyThreads + threadIdx.x;
-      if (v < pl.vpp) *reinterpret_cast<V*>(d + off[u]) = x[u];
-    }
+  if (pl.cpp) {
+    copy_chunks(pl, step, count, pair);
     return;
   }
-  // Several small pages.
-  const uint32_t n = (uint32_t)min((int64_t)pl.ppw, count - step * pl.ppw) * pl.vpp;
-  for (uint32_t l = threadIdx.x; l < n; l += kCopyThreads) {
-    const uint32_t k = l / pl.vpp;
-    int src, dst;
-    if (!pair(step * pl.ppw + k, src, dst)) continue;
-    const int64_t off = plane_offset(pl, l - k * pl.vpp);
-    copy_vec<V>(pl.base + (int64_t)src * pl.page + off, pl.base + (int64_t)dst * pl.page + off);
-  }
-}
-
-__device__ __forceinline__ int64_t plane_steps(const Plane& pl, int64_t count) {
-  return pl.ppw == 1 ? count * pl.spp : (count + pl.ppw - 1) / pl.ppw;
-}
-
-template <typename Pair>
-__device__ __forceinline__ void copy_step_any(const Plane& pl, int64_t step, int64_t count, Pair pair) {
   switch (pl.log2v) {
-    case 4: copy_step<u32x4>(pl, step, count, pair); break;
-    case 3: copy_step<u32x2>(pl, step, count, pair); break;
-    case 2: copy_step<u32>(pl, step, count, pair); break;
-    case 1: copy_step<uint16_t>(pl, step, count, pair); break;
-    default: copy_step<uint8_t>(pl, step, count, pair); break;
+    case 4: copy_vectors<u32x4>(pl, step, count, pair); break;
+    case 3: copy_vectors<u32x2>(pl, step, count, pair); break;
+    case 2: copy_vectors<u32>(pl, step, count, pair); break;
+    case 1: copy_vectors<uint16_t>(pl, step, count, pair); break;
+    default: copy_vectors<uint8_t>(pl, step, count, pair); break;
   }
 }
 
 // blockIdx.y: plane; blockIdx.x: steps of it, the grid's width apart.
-__global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(const Planes planes, const int32_t* __restrict__ src,
-                                                                  const int32_t* __restrict__ dst, int64_t count) {
+__global__ __launch_bounds__(kCopyThreads, 8) void copy_pages_kernel(const Planes planes,
+                                                                                  const int32_t* __restrict__ src,
+                                                                                  const int32_t* __restrict__ dst,
+                                                                                  int64_t count) {
   const Plane pl = planes.p[blockIdx.y];
   const int64_t steps = plane_steps(pl, count);
   for (int64_t step = blockIdx.x; step < steps; step += gridDim.x)
-    copy_step_any(pl, step, count, [&](int64_t i, int& s, int& d) {
+    copy_step(pl, step, count, [&](int64_t i, int& s, int& d) {
       s = src[i];
       d = dst[i];
       return (unsigned)s < (unsigned)planes.num_pages && (unsigned)d < (unsigned)planes.num_pages;
@@ -138,7 +168,8 @@ struct ForkParams {
 // blockIdx.y: the fork; blockIdx.z: a plane of its last page, or (the last) its
 // table row; blockIdx.x: steps.  Every workgroup of a fork reads only its
 // parent's row, which no fork of the call writes, and decides alike.
-__global__ __launch_bounds__(kCopyThreads) void fork_kernel(const ForkParams p) {
+__global__ __launch_bounds__(kCopyThreads, 8) void fork_kernel(const ForkParams p) {
+  if ((int)blockIdx.z < p.planes.n && (int64_t)blockIdx.x >= plane_steps(p.planes.p[blockIdx.z], 1)) return;
   const int i = blockIdx.y;
   const int parent = p.parents[i], child = p.children[i];
   if ((unsigned)parent >= (unsigned)p.B || (unsigned)child >= (unsigned)p.B || parent == child) return;
@@ -167,7 +198,7 @@ __global__ __launch_bounds__(kCopyThreads) void fork_kernel(const ForkParams p) 
   const Plane pl = p.planes.p[blockIdx.z];
   const int64_t steps = plane_steps(pl, 1);
   for (int64_t step = blockIdx.x; step < steps; step += gridDim.x)
-    copy_step_any(pl, step, 1, [&](int64_t, int& s, int& d) {
+    copy_step(pl, step, 1, [&](int64_t, int& s, int& d) {
       s = src;
       d = dst;
       return true;
@@ -237,8 +268,9 @@ __global__ __launch_bounds__(kUseThreads) void use_mark_kernel(const UseParams p
 }
 
 // Sum over the workgroup (all threads get it) and the sum over the threads before.
+template <int THREADS = kUseThreads>
 __device__ __forceinline__ int use_scan(int x, int& before) {
-  __shared__ int s[kUseThreads / 64];
+  __shared__ int s[THREADS / 64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int y = x;
 #pragma unroll
@@ -252,7 +284,7 @@ __device__ __forceinline__ int use_scan(int x, int& before) {
   int total = 0;
   before = y - x;
 #pragma unroll
-  for (int k = 0; k < kUseThreads / 64; ++k) {
+  for (int k = 0; k < THREADS / 64; ++k) {
     before += k < w ? s[k] : 0;
     total += s[k];
   }
@@ -330,15 +362,85 @@ __global__ __launch_bounds__(kUseThreads) void use_list_kernel(const UseParams p
   }
 }
 
+// The four launches above in one workgroup, for small pools and tables: the
+// flags are bits in LDS, whose popcounts are scanned; id i's rank is that of its
+// word and of the bits below it.
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallPages = 1 << 16;    // ids
+constexpr int kSmallEntries = 1 << 15;  // table entries
+
+template <bool COMPACT>
+__global__ __launch_bounds__(kSmallThreads) void use_small_kernel(const UseParams p) {
+  constexpr int kWords = kSmallPages / 32, kEach = kWords / kSmallThreads;
+  __shared__ uint32_t bits[kWords];
+  __shared__ int before[kWords];
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) bits[tid * kEach + k] = 0;
+  for (int i = tid; i < p.nrows; i += kSmallThreads) {
+    const int b = p.rows[i];
+    if ((unsigned)b >= (unsigned)p.B) continue;
+    p.lens[b] = 0;
+    if (p.held) p.held[b] = 0;
+  }
+  __syncthreads();  // the rows' lengths too: one workgroup shares its L1
+  constexpr int kWaves = kSmallThreads / 64;
+  const int wave = tid >> 6, lane = tid & 63;
+  const int per_row = max(1, kWaves / max(p.B, 1));
+  for (int u = wave; u < p.B * per_row; u += kWaves) {
+    const int b = u / per_row;
+    const int cols = used_columns(p, b);
+    const int32_t* row = p.pt + (int64_t)b * p.pt_sb;
+#pragma unroll 4
+    for (int c = (u - b * per_row) * 64 + lane; c < cols; c += per_row * 64) {
+      const int id = row[c];
+      if ((unsigned)id < (unsigned)p.num_pages) atomicOr(bits + (id >> 5), 1u << (id & 31));
+    }
+  }
+  __syncthreads();
+  int x = 0, at;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) x += __popc(bits[tid * kEach + k]);
+  const int n = use_scan<kSmallThreads>(x, at);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    before[tid * kEach + k] = at;
+    at += __popc(bits[tid * kEach + k]);
+  }
+  __syncthreads();
+  auto rank = [&](int id) { return before[id >> 5] + __popc(bits[id >> 5] & ((1u << (id & 31)) - 1)); };
+  const int below = COMPACT && n < p.num_pages ? rank(n) : n;  // used ids below n
+  if (tid == 0) {
+    *p.total = COMPACT ? n : p.num_pages - n;
+    if constexpr (COMPACT) p.counts[(p.num_pages + kUseGroup - 1) / kUseGroup] = n - below;  // moves
+  }
+  for (int id = tid; id < p.num_pages; id += kSmallThreads) {
+    const bool used = (bits[id >> 5] >> (id & 31)) & 1;
+    const int r = rank(id);
+    if constexpr (COMPACT) {
+      if (!used && id < n) p.list[id - r] = id;
+      if (used && id >= n) {
+        p.src[r - below] = id;
+        p.rank[id] = r - below;
+      } else {
+        p.remap[id] = used ? id : -1;
+      }
+    } else {
+      if (!used) p.list[id - r] = id;
+      else p.list[p.num_pages - n + r] = -1;
+    }
+  }
+}
+
 // The moves: blockIdx.y < n planes: copies of that plane; the last: new ids.
-__global__ __launch_bounds__(kCopyThreads) void compact_apply_kernel(const Planes planes, const UseParams p,
+__global__ __launch_bounds__(kCopyThreads, 8) void compact_apply_kernel(const Planes planes, const UseParams p,
                                                                      int groups) {
   const int moves = p.counts[groups];
   if ((int)blockIdx.y < planes.n) {
     const Plane pl = planes.p[blockIdx.y];
     const int64_t steps = plane_steps(pl, moves);
     for (int64_t step = blockIdx.x; step < steps; step += gridDim.x)
-      copy_step_any(pl, step, moves, [&](int64_t i, int& s, int& d) {
+      copy_step(pl, step, moves, [&](int64_t i, int& s, int& d) {
         s = p.src[i];
         d = p.list[i];
         return true;
@@ -412,8 +514,9 @@ fat::Plane make_plane(void* base, int64_t page, int64_t slots, int64_t slot_stri
   p.inner = (uint32_t)inner;
   p.vpr = (uint32_t)(row >> log2v);
   p.vpp = (uint32_t)(outer * inner * (row >> log2v));
-  p.ppw = std::max<uint32_t>(1, fat::kCopyStep / p.vpp);
-  p.spp = (p.vpp + fat::kCopyStep - 1) / fat::kCopyStep;
+  p.inv = p.vpp > 1 ? (uint32_t)((uint64_t(1) << 32) / p.vpp) : 0;
+  const uint64_t run = (uint64_t)p.vpp << log2v;
+  p.cpp = log2v == 4 && p.vpr == p.vpp && run % fat::kChunk == 0 ? (uint32_t)(run / fat::kChunk) : 0;
   p.log2v = log2v;
   return p;
 }
@@ -466,16 +569,20 @@ int make_planes(const fat_pool& a, fat::Planes* out, const char* who) {
 }
 
 int64_t host_steps(const fat::Plane& p, int64_t count) {
-  return p.ppw == 1 ? count * p.spp : (count + p.ppw - 1) / p.ppw;
+  return p.cpp ? (count * p.cpp + fat::kStepChunks - 1) / fat::kStepChunks
+               : (count * p.vpp + fat::kStepVectors - 1) / fat::kStepVectors;
 }
 
 // Workgroups (of 256 threads) that fill the chip: 8 per CU.
 constexpr int64_t kFullGrid = 8 * 256;
+// A workgroup per step where the number of steps is known (2 % over kFullGrid's
+// loops), within a launch's limit of 2^32 threads.
+constexpr int64_t kWideGrid = 1 << 22;
 
-unsigned copy_grid(const fat::Planes& pl, int64_t count) {
+unsigned copy_grid(const fat::Planes& pl, int64_t count, int64_t limit = kFullGrid) {
   int64_t most = 1;
   for (int i = 0; i < pl.n; ++i) most = std::max(most, host_steps(pl.p[i], count));
-  return (unsigned)std::min(most, kFullGrid);
+  return (unsigned)std::min(most, limit);
 }
 
 int64_t use_groups(int64_t num_pages) { return (num_pages + fat::kUseGroup - 1) / fat::kUseGroup; }
@@ -512,8 +619,14 @@ bool use_args_ok(const void* lens, const void* pt, int64_t pt_sb, int batch, int
   return true;
 }
 
-// Flags and counts of the pages in use.
+// The pages in use, and the lists of them.  One workgroup where it has at most
+// 32 table entries and 64 ids per thread, else four launches (each some 2 us).
+template <bool COMPACT>
 int launch_use(const fat::UseParams& p, hipStream_t stream) {
+  if (p.num_pages <= fat::kSmallPages && (int64_t)p.B * p.max_pages <= fat::kSmallEntries) {
+    hipLaunchKernelGGL((fat::use_small_kernel<COMPACT>), dim3(1), dim3(fat::kSmallThreads), 0, stream, p);
+    return fat_host::launch_status("use_small_kernel");
+  }
   const int64_t groups = use_groups(p.num_pages);
   const int64_t words = groups * fat::kUseGroup / 16;
   const int64_t most = std::max<int64_t>(words, p.nrows);
@@ -528,7 +641,9 @@ int launch_use(const fat::UseParams& p, hipStream_t stream) {
     if ((rc = fat_host::launch_status("use_mark_kernel")) != FAT_OK) return rc;
   }
   hipLaunchKernelGGL(fat::use_count_kernel, dim3((unsigned)groups), dim3(fat::kUseThreads), 0, stream, p);
-  return fat_host::launch_status("use_count_kernel");
+  if ((rc = fat_host::launch_status("use_count_kernel")) != FAT_OK) return rc;
+  hipLaunchKernelGGL((fat::use_list_kernel<COMPACT>), dim3((unsigned)groups), dim3(fat::kUseThreads), 0, stream, p);
+  return fat_host::launch_status("use_list_kernel");
 }
 
 }  // namespace
@@ -553,8 +668,9 @@ extern "C" int fat_copy_pages(const fat_copy_pages_args* a, void* stream_ptr) {
     return FAT_E_INVALID;
   }
   if (a->count == 0) return FAT_OK;
-  hipLaunchKernelGGL(fat::copy_pages_kernel, dim3(copy_grid(planes, a->count), planes.n), dim3(fat::kCopyThreads), 0,
-                     static_cast<hipStream_t>(stream_ptr), planes, a->src, a->dst, a->count);
+  const dim3 grid(copy_grid(planes, a->count, kWideGrid), planes.n), block(fat::kCopyThreads);
+  hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+  hipLaunchKernelGGL(fat::copy_pages_kernel, grid, block, 0, stream, planes, a->src, a->dst, a->count);
   return fat_host::launch_status("copy_pages_kernel");
 }
 
@@ -589,7 +705,8 @@ extern "C" int fat_fork_sequences(const fat_fork_args* a, void* stream_ptr) {
   prm.P = a->pool.page_size;
   const unsigned table = (unsigned)std::min<int64_t>((a->max_pages + 1023) / 1024, 64);
   const dim3 grid(std::max(copy_grid(prm.planes, 1), table), (unsigned)a->count, prm.planes.n + 1);
-  hipLaunchKernelGGL(fat::fork_kernel, grid, dim3(fat::kCopyThreads), 0, static_cast<hipStream_t>(stream_ptr), prm);
+  hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+  hipLaunchKernelGGL(fat::fork_kernel, grid, dim3(fat::kCopyThreads), 0, stream, prm);
   return fat_host::launch_status("fork_kernel");
 }
 
@@ -621,11 +738,7 @@ extern "C" int fat_free_sequences(const fat_free_args* a, void* stream_ptr) {
   prm.list = a->pages;
   prm.total = a->num_free;
   hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
-  const int rc = launch_use(prm, stream);
-  if (rc != FAT_OK) return rc;
-  hipLaunchKernelGGL((fat::use_list_kernel<false>), dim3((unsigned)use_groups(a->num_pages)), dim3(fat::kUseThreads), 0,
-                     stream, prm);
-  return fat_host::launch_status("use_list_kernel");
+  return launch_use<false>(prm, stream);
 }
 
 extern "C" int fat_compact_pages(const fat_compact_args* a, void* stream_ptr) {
@@ -653,14 +766,12 @@ extern "C" int fat_compact_pages(const fat_compact_args* a, void* stream_ptr) {
   prm.remap = a->remap;
   prm.total = a->num_used;
   hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
-  if ((rc = launch_use(prm, stream)) != FAT_OK) return rc;
+  if ((rc = launch_use<true>(prm, stream)) != FAT_OK) return rc;
   const int groups = (int)use_groups(prm.num_pages);
-  hipLaunchKernelGGL((fat::use_list_kernel<true>), dim3((unsigned)groups), dim3(fat::kUseThreads), 0, stream, prm);
-  if ((rc = fat_host::launch_status("use_list_kernel")) != FAT_OK) return rc;
   // At most half of the pages move; the number is known on the device only.
   const unsigned wide = std::max(copy_grid(planes, prm.num_pages / 2 + 1),
                                  (unsigned)std::min<int64_t>(std::max(prm.B, 1), kFullGrid));
-  hipLaunchKernelGGL(fat::compact_apply_kernel, dim3(wide, planes.n + 1), dim3(fat::kCopyThreads), 0, stream, planes,
-                     prm, groups);
+  const dim3 grid(wide, planes.n + 1), block(fat::kCopyThreads);
+  hipLaunchKernelGGL(fat::compact_apply_kernel, grid, block, 0, stream, planes, prm, groups);
   return fat_host::launch_status("compact_apply_kernel");
 }

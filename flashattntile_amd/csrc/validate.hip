@@ -119,7 +119,6 @@ struct CheckParams {
   const float* values;
   int64_t count;
   const int32_t* ids[3];
-  int32_t* scratch;
   int32_t num_pages;
   int32_t tokens;
 };
@@ -150,7 +149,7 @@ __device__ __forceinline__ long long check_reduce(long long x) {
 // so no cache is written back and the host needs no synchronisation.
 template <int KIND>
 __global__ __launch_bounds__(kCheckThreads) void check_kernel(const CheckParams p) {
-  constexpr bool TABLE = KIND == FAT_CHECK_CACHE || KIND == FAT_CHECK_PAGED || KIND == FAT_CHECK_FREE;
+  constexpr bool TABLE = KIND == FAT_CHECK_CACHE || KIND == FAT_CHECK_PAGED;
   constexpr bool LENS = TABLE || KIND == FAT_CHECK_APPEND;
   constexpr bool CU = KIND == FAT_CHECK_VARLEN || KIND == FAT_CHECK_PAGED;
   const int tid = threadIdx.x;
@@ -232,11 +231,6 @@ __global__ __launch_bounds__(kCheckThreads) void check_kernel(const CheckParams 
       mk = check_reduce<RMax>(mk);
       keyless = check_reduce<RMin>(keyless);
     }
-    if constexpr (KIND == FAT_CHECK_FREE) {
-      for (int64_t i = tid; i < p.count; i += kCheckThreads) flags |= (unsigned)p.ids[0][i] >= (unsigned)p.B ? 1 : 0;
-      flags = check_reduce<ROr>(flags);
-      if (tid == 0) put(7, flags);
-    }
     if (tid == 0) {
       put(0, mn);
       put(1, mx);
@@ -267,175 +261,253 @@ __global__ __launch_bounds__(kCheckThreads) void check_kernel(const CheckParams 
   }
 }
 
-// SHARED: workgroup x takes rows x, x + gridDim.x, ..: the page range of their
-// used columns, and whether those that the prefix fills name the pages of the
-// group's first row (else INT_MIN for the smallest id).  Workgroup 0 also
-// reduces lengths, offsets and prefixes.
-__global__ __launch_bounds__(kCheckThreads) void check_shared_kernel(const CheckParams p) {
+// FREE and SHARED: workgroup 0 reduces the lengths (and the rows to free, the
+// groups, their prefixes), the others' waves take the table: FREE's as CACHE
+// does, SHARED's used columns, with a comparison of those that a prefix fills with
+// the group's first row (a difference makes the smallest id INT_MIN).  A row's
+// columns go to `per_row` waves in turn, so no entry costs a division and few
+// long rows spread as well as many short ones.
+constexpr int kRowsThreads = 1024;
+constexpr int kRowsWaves = kRowsThreads / 64;
+constexpr int64_t kRowsEntries = 4096;  // table entries per workgroup
+
+// Reduces the first `waves` waves' x[0 .. N - 1] (x[i] by op[i]): all of a wave's
+// shuffles overlap, and the workgroup synchronises once.  Threads i < N return
+// the i-th.  (Waves without an element shuffle nothing: sixteen waves' took 4 us
+// of a check's 11.)
+enum RowOp : int { kMin, kMax, kSum, kOr };
+template <int N>
+__device__ __forceinline__ long long rows_reduce(long long (&x)[N], const RowOp (&op)[N], int waves) {
+  __shared__ long long s[kRowsWaves][N];
+  auto f = [](RowOp o, long long a, long long b) {
+    return o == kMin ? (a < b ? a : b) : o == kMax ? (a > b ? a : b) : o == kSum ? a + b : (a | b);
+  };
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave < waves) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = f(op[i], x[i], __shfl_xor(x[i], off));
+    }
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[wave][i] = x[i];
+    }
+  }
+  __syncthreads();
+  long long r = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if ((int)threadIdx.x == i) {
+      r = s[0][i];
+      for (int w = 1; w < waves; ++w) r = f(op[i], r, s[w][i]);
+    }
+  }
+  return r;
+}
+
+template <int KIND>
+__global__ __launch_bounds__(kRowsThreads) void check_rows_kernel(const CheckParams p) {
+  constexpr bool SHARED = KIND == FAT_CHECK_SHARED;
   const int tid = threadIdx.x;
   const int G = (int)p.count;
   const int32_t* prefix = p.ids[0];
-  auto group_of = [&](int b) {  // the largest g with cu_q[g] <= b, -1: none
-    int lo = -1, hi = G;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.cu_q[mid] <= b) lo = mid;
-      else hi = mid;
-    }
-    return lo;
-  };
   auto put = [&](int word, long long v) {
     __hip_atomic_store(p.host + word, (int64_t)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   };
-  int pmn = INT_MAX, pmx = INT_MIN;
-  bool differs = false;
-  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {  // uniform
-    const int g = group_of(b);
-    const int lead = g < 0 ? b : max(p.cu_q[g], 0);
-    const long long len = max(p.lens[b], 0);
-    const int cols = (int)min((len + p.P - 1) / p.P, (long long)p.max_pages);
-    const int same = lead == b ? 0 : min(max(prefix[g], 0) / p.P, cols);
-    const int32_t* row = p.pt + b * p.pt_sb;
-    const int32_t* first = p.pt + lead * p.pt_sb;
-#pragma unroll 4
-    for (int c = tid; c < cols; c += kCheckThreads) {
-      const int id = row[c];
-      pmn = min(pmn, id);
-      pmx = max(pmx, id);
-      if (c < same) differs |= first[c] != id;
-    }
-  }
-  pmn = (int)check_reduce<RMin>(differs ? INT_MIN : pmn);
-  pmx = (int)check_reduce<RMax>(pmx);
+  auto pages_of = [&](int len) { return (int)(((unsigned)max(len, 0) + (unsigned)p.P - 1) / (unsigned)p.P); };
+  long long range[2] = {INT_MAX, INT_MIN};
+  const RowOp range_op[2] = {kMin, kMax};
+  const int workers = ((int)gridDim.x - 1) * kRowsWaves;
   if (blockIdx.x == 0) {  // uniform
-    long long mn = INT_MAX, mx = INT_MIN, pages = 0, flags = 0, most = 0, longest = 0, behind = 0, sum_p = 0,
-              sum_own = 0, sum_rows = 0;
-    for (int b = tid; b < p.B; b += kCheckThreads) {
-      const long long len = p.lens[b];
-      const int g = group_of(b);
-      const long long n = g < 0 ? 0 : prefix[g];
-      mn = min(mn, len);
-      mx = max(mx, len);
-      pages += (max(len, 0ll) + p.P - 1) / p.P;
-      if (n > len - p.tokens + 1) flags |= 4;
-      behind = max(behind, len - n);
-      sum_own += len - n;
-    }
-    for (int g = tid; g < G; g += kCheckThreads) {
-      const long long seqs = (long long)p.cu_q[g + 1] - p.cu_q[g];
-      flags |= (seqs < 0 ? 1 : 0) | (prefix[g] < 0 ? 2 : 0);
-      most = max(most, seqs);
-      if (seqs > 0) {
-        longest = max(longest, (long long)prefix[g]);
-        sum_p += prefix[g];
-        sum_rows += prefix[g] * seqs;
+    if constexpr (SHARED) {
+      // min and max length, pages, flags, sequences of a group, prefix, keys behind it, and three sums
+      long long x[10] = {INT_MAX, INT_MIN, 0, 0, 0, 0, 0, 0, 0, 0};
+      const RowOp op[10] = {kMin, kMax, kSum, kOr, kMax, kMax, kMax, kSum, kSum, kSum};
+      for (int b = tid; b < p.B; b += kRowsThreads) {
+        const long long len = p.lens[b];
+        int g = -1, hi = G;  // the largest g with cu_q[g] <= b, if any
+        while (hi - g > 1) {
+          const int mid = (g + hi) >> 1;
+          if (p.cu_q[mid] <= b) g = mid;
+          else hi = mid;
+        }
+        const long long n = g < 0 ? 0 : prefix[g];
+        x[0] = min(x[0], len);
+        x[1] = max(x[1], len);
+        x[2] += pages_of((int)len);
+        x[3] |= n > len - p.tokens + 1 ? 4 : 0;
+        x[6] = max(x[6], len - n);
+        x[8] += len - n;
+      }
+      for (int g = tid; g < G; g += kRowsThreads) {
+        const long long seqs = (long long)p.cu_q[g + 1] - p.cu_q[g], n = prefix[g];
+        x[3] |= (seqs < 0 ? 1 : 0) | (n < 0 ? 2 : 0);
+        x[4] = max(x[4], seqs);
+        if (seqs > 0) {
+          x[5] = max(x[5], n);
+          x[7] += n;
+          x[9] += n * seqs;
+        }
+      }
+      const long long r = rows_reduce(x, op, (int)min((max((int64_t)p.B, p.count) + 63) / 64, (int64_t)kRowsWaves));
+      const int word[10] = {0, 1, 2, 7, 5, 6, 8, 9, 10, 11};
+#pragma unroll
+      for (int i = 0; i < 10; ++i) {
+        if (tid == i) put(word[i], r);
+      }
+      if (tid == 0) {
+        put(3, p.cu_q[0]);
+        put(4, p.cu_q[G]);
+      }
+    } else {
+      long long x[4] = {INT_MAX, INT_MIN, 0, 0};
+      const RowOp op[4] = {kMin, kMax, kSum, kOr};
+      for (int b = tid; b < p.B; b += kRowsThreads) {
+        const long long len = p.lens[b];
+        x[0] = min(x[0], len);
+        x[1] = max(x[1], len);
+        x[2] += pages_of((int)len);
+      }
+      for (int64_t i = tid; i < p.count; i += kRowsThreads) x[3] |= (unsigned)p.ids[0][i] >= (unsigned)p.B ? 1 : 0;
+      const long long r = rows_reduce(x, op, (int)min((max((int64_t)p.B, p.count) + 63) / 64, (int64_t)kRowsWaves));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (tid == i) put(i < 3 ? i : 7, r);
       }
     }
-    mn = check_reduce<RMin>(mn);
-    mx = check_reduce<RMax>(mx);
-    pages = check_reduce<RSum>(pages);
-    flags = check_reduce<ROr>(flags);
-    most = check_reduce<RMax>(most);
-    longest = check_reduce<RMax>(longest);
-    behind = check_reduce<RMax>(behind);
-    sum_p = check_reduce<RSum>(sum_p);
-    sum_own = check_reduce<RSum>(sum_own);
-    sum_rows = check_reduce<RSum>(sum_rows);
-    if (tid == 0) {
-      put(0, mn);
-      put(1, mx);
-      put(2, pages);
-      put(3, p.cu_q[0]);
-      put(4, p.cu_q[G]);
-      put(5, most);
-      put(6, longest);
-      put(7, flags);
-      put(8, behind);
-      put(9, sum_p);
-      put(10, sum_own);
-      put(11, sum_rows);
+  } else {
+    const int lane = tid & 63;
+    const int worker = ((int)blockIdx.x - 1) * kRowsWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int per_row = max(1, workers / p.B);
+    int need = 0;
+    if constexpr (!SHARED) {
+      int mx = 0;
+      for (int b = lane; b < p.B; b += 64) mx = max(mx, p.lens[b]);
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) mx = max(mx, __shfl_xor(mx, off));
+      need = __builtin_amdgcn_readfirstlane(min(pages_of(mx), p.max_pages));
     }
+    int pmn = INT_MAX, pmx = INT_MIN;
+    bool differs = false;
+    for (long long u = worker; u < (long long)p.B * per_row; u += workers) {
+      const int b = (int)(u / per_row);
+      const int32_t* row = p.pt + b * p.pt_sb;
+      const int32_t* first = row;
+      int cols = need, same = 0;
+      if constexpr (SHARED) {
+        // The largest g with cu_q[g] <= b, if any: 64 samples at a time.
+        int g = -1;
+        for (long long lo = 0, n = G; n > 0;) {
+          const long long step = (n + 63) / 64;
+          const long long at = lo + lane * step;
+          const unsigned long long below = __ballot(at < lo + n && p.cu_q[at < lo + n ? at : lo] <= b);
+          if (!below) break;
+          g = (int)(lo + (63 - __clzll(below)) * step);
+          n = min(step, lo + n - g) - 1;
+          lo = g + 1;
+        }
+        const int lead = g < 0 ? b : max(p.cu_q[g], 0);
+        cols = min(pages_of(p.lens[b]), p.max_pages);
+        same = lead == b ? 0 : min(max(prefix[g], 0) / p.P, cols);
+        first = p.pt + lead * p.pt_sb;
+      }
+      const int stride = per_row * 64;
+#pragma unroll 8
+      for (long long c = (u - (long long)b * per_row) * 64 + lane; c < cols; c += stride) {
+        const int id = row[c];
+        pmn = min(pmn, id);
+        pmx = max(pmx, id);
+        if constexpr (SHARED) {
+          if (c < same) differs |= first[c] != id;
+        }
+      }
+    }
+    range[0] = differs ? INT_MIN : pmn;
+    range[1] = pmx;
+    const long long r = rows_reduce(range, range_op, kRowsWaves);
+    range[0] = r;
+    range[1] = __shfl(r, 1);
   }
-  if (tid == 0) {
+  if (tid < 64) {  // the wave whose results the tickets follow
     const int at = FAT_CHECK_RESULTS + 2 * blockIdx.x;
-    put(at, (long long)(((unsigned long long)(uint32_t)pmx << 32) | (uint32_t)pmn));
+    if (tid == 0) put(at, (long long)(((unsigned long long)(uint32_t)range[1] << 32) | (uint32_t)range[0]));
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the results are complete
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    put(at + 1, p.ticket);
+    if (tid == 0) put(at + 1, p.ticket);
   }
 }
 
-// COPY and FORK: ranges, and ids that are given twice or on both sides.  An id
-// d of list b is "owned" by the last writer of own[d], and own needs no
-// clearing: own[x] names an element k only if 0 <= k < count and b[k] == x, so
-// what memory held before never counts.  One workgroup (its threads have to see
-// each other's stores); 8192 pairs take as long as the launch itself.
+// COPY and FORK: ranges, and ids that are given twice or on both sides.  One
+// workgroup marks a list's ids in a bitmap in LDS, 2^19 ids at a time (a pool of
+// more takes several turns over the list): the bit that was there before is a
+// repetition, and the other list's ids are looked up in it.
 constexpr int kListThreads = 1024;
-
-__device__ __forceinline__ int own_load(const int32_t* own, int x) {
-  return __hip_atomic_load(own + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void own_store(int32_t* own, int x, int k) {
-  __hip_atomic_store(own + x, k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-// Whether x is an element of list b[0 .. n - 1], by the owners.
-__device__ __forceinline__ bool owned(const int32_t* own, const int32_t* b, int64_t n, int x) {
-  const int k = own_load(own, x);
-  return (unsigned)k < (unsigned)n && b[k] == x;
-}
+constexpr int kListIds = 1 << 19;
 
 template <int KIND>
 __global__ __launch_bounds__(kListThreads) void check_lists_kernel(const CheckParams p) {
   constexpr bool FORK = KIND == FAT_CHECK_FORK;
+  __shared__ uint32_t bits[kListIds / 32];
+  __shared__ int s_flags;
   const int tid = threadIdx.x;
   const int n = (int)p.count;
   const int32_t* a = p.ids[0];
   const int32_t* b = p.ids[1];
   const int32_t* pages = p.ids[2];
-  const unsigned limit = FORK ? p.B : p.num_pages;
-  int32_t* own = p.scratch;                    // [limit]
-  int32_t* own_pages = p.scratch + p.B;        // FORK: [num_pages]
+  const int limit = FORK ? p.B : p.num_pages;
   int flags = 0;
+  if (tid == 0) s_flags = 0;
+  auto clear = [&](int ids) {
+    __syncthreads();
+    for (int i = tid; i < (ids + 31) / 32; i += kListThreads) bits[i] = 0;
+    __syncthreads();
+  };
+  auto mark = [&](unsigned x) { return (atomicOr(bits + (x >> 5), 1u << (x & 31)) >> (x & 31)) & 1; };
   // FORK: whether fork i's parent ends inside a page (its pages[i] is used).
   auto tail = [&](int i, int& len) {
     const int parent = a[i];
-    len = (unsigned)parent < limit ? p.lens[parent] : 0;
+    len = (unsigned)parent < (unsigned)limit ? p.lens[parent] : 0;
     return len > 0 && len <= (int64_t)p.max_pages * p.P && len % p.P != 0;
   };
-#pragma unroll 4
-  for (int i = tid; i < n; i += kListThreads) {
-    const int x = a[i], y = b[i];
-    flags |= (unsigned)x >= limit ? 1 : 0;
-    if ((unsigned)y >= limit) flags |= 2;
-    else own_store(own, y, i);
-    if constexpr (FORK) {
+  for (int base = 0; base < limit; base += min(kListIds, limit - base)) {
+    const unsigned ids = min(kListIds, limit - base);
+    clear(ids);
+#pragma unroll 8
+    for (int i = tid; i < n; i += kListThreads) {
+      const int y = b[i];
+      if ((unsigned)y >= (unsigned)limit) flags |= 2;
+      else if ((unsigned)(y - base) < ids && mark(y - base)) flags |= 4;
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int i = tid; i < n; i += kListThreads) {
+      const int x = a[i];
+      if ((unsigned)x >= (unsigned)limit) flags |= 1;
+      else if ((unsigned)(x - base) < ids && ((bits[(x - base) >> 5] >> ((x - base) & 31)) & 1)) flags |= 8;
+    }
+  }
+  if constexpr (FORK) {
+    for (int i = tid; i < n; i += kListThreads) {
+      const int x = a[i], y = b[i];
       int len;
-      if ((unsigned)y < limit && p.lens[y] != 0) flags |= 16;
+      if ((unsigned)y < (unsigned)limit && p.lens[y] != 0) flags |= 16;
       if (tail(i, len)) {
         if ((unsigned)p.pt[x * p.pt_sb + len / p.P] >= (unsigned)p.num_pages) flags |= 64;
         if ((unsigned)pages[i] >= (unsigned)p.num_pages) flags |= 128;
-        else own_store(own_pages, pages[i], i);
       }
       if (len < 0 || len > (int64_t)p.max_pages * p.P) flags |= 32;
     }
-  }
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's stores are complete
-  __syncthreads();
-#pragma unroll 4
-  for (int i = tid; i < n; i += kListThreads) {
-    const int x = a[i], y = b[i];
-    if ((unsigned)y < limit && own_load(own, y) != i) flags |= 4;
-    if ((unsigned)x < limit && owned(own, b, n, x)) flags |= 8;
-    if constexpr (FORK) {
-      int len;
-      if (tail(i, len) && (unsigned)pages[i] < (unsigned)p.num_pages && own_load(own_pages, pages[i]) != i)
-        flags |= 256;
+    for (int base = 0; base < p.num_pages; base += min(kListIds, p.num_pages - base)) {
+      const unsigned ids = min(kListIds, p.num_pages - base);
+      clear(ids);
+      for (int i = tid; i < n; i += kListThreads) {
+        int len;
+        if (tail(i, len) && (unsigned)(pages[i] - base) < ids && mark(pages[i] - base)) flags |= 256;
+      }
     }
   }
-  __shared__ int s_flags;
-  if (tid == 0) s_flags = 0;
   __syncthreads();
   if (flags) atomicOr(&s_flags, flags);
   __syncthreads();
@@ -459,7 +531,10 @@ int check_groups(const fat_check_args* a) {
   if (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_APPEND || a->kind == FAT_CHECK_COPY ||
       a->kind == FAT_CHECK_FORK)
     return 1;
-  if (a->kind == FAT_CHECK_SHARED) return std::min(a->batch, FAT_CHECK_MAX_GROUPS);
+  if (a->kind == FAT_CHECK_SHARED || a->kind == FAT_CHECK_FREE) {
+    const int64_t n = ((int64_t)a->batch * a->max_pages + fat::kRowsEntries - 1) / fat::kRowsEntries;
+    return (int)std::min<int64_t>(1 + std::max<int64_t>(n, 1), FAT_CHECK_MAX_GROUPS);
+  }
   const int64_t entries = a->kind == FAT_CHECK_RANGE ? a->count : (int64_t)a->batch * a->max_pages;
   const int64_t n = (entries + fat::kCheckEntries - 1) / fat::kCheckEntries;
   return (int)std::min<int64_t>(std::max<int64_t>(n, 1), FAT_CHECK_MAX_GROUPS);
@@ -472,7 +547,7 @@ bool check_args_ok(const fat_check_args* a, const char* who) {
   const bool copy = a && a->kind == FAT_CHECK_COPY, fork = a && a->kind == FAT_CHECK_FORK;
   const bool lens = a && a->kind != FAT_CHECK_VARLEN && !range && !copy;
   const bool ids = copy || fork || shared || (a && a->kind == FAT_CHECK_FREE && a->count > 0);
-  if (!a || !a->host || (ids && !a->ids[0]) || ((copy || fork) && (!a->ids[1] || !a->scratch)) ||
+  if (!a || !a->host || (ids && !a->ids[0]) || ((copy || fork) && !a->ids[1]) ||
       (fork && !a->ids[2]) || (cu && !a->cu_q) || (a->kind == FAT_CHECK_VARLEN && !a->cu_k) || (lens && !a->seq_lens) ||
       (lens && !a->page_table) || (range && !a->values)) {
     fat_host::set_error("%s: a required pointer is NULL", who);
@@ -508,15 +583,19 @@ extern "C" int fat_check_begin(const fat_check_args* a, void* stream_ptr) {
   }
   const fat::CheckParams prm{a->cu_q, a->cu_k, a->seq_lens, a->page_table, a->page_table_stride, a->host,
                              a->ticket, a->batch, a->max_pages, a->page_size, a->values, a->count,
-                             {a->ids[0], a->ids[1], a->ids[2]}, a->scratch, a->num_pages, a->tokens};
+                             {a->ids[0], a->ids[1], a->ids[2]}, a->num_pages, a->tokens};
   const dim3 grid((unsigned)check_groups(a)), block(fat::kCheckThreads);
   switch (a->kind) {
     case FAT_CHECK_CACHE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_CACHE>), grid, block, 0, stream, prm); break;
     case FAT_CHECK_VARLEN: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_VARLEN>), grid, block, 0, stream, prm); break;
     case FAT_CHECK_PAGED: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_PAGED>), grid, block, 0, stream, prm); break;
     case FAT_CHECK_RANGE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_RANGE>), grid, block, 0, stream, prm); break;
-    case FAT_CHECK_FREE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_FREE>), grid, block, 0, stream, prm); break;
-    case FAT_CHECK_SHARED: hipLaunchKernelGGL(fat::check_shared_kernel, grid, block, 0, stream, prm); break;
+    case FAT_CHECK_FREE:
+      hipLaunchKernelGGL((fat::check_rows_kernel<FAT_CHECK_FREE>), grid, dim3(fat::kRowsThreads), 0, stream, prm);
+      break;
+    case FAT_CHECK_SHARED:
+      hipLaunchKernelGGL((fat::check_rows_kernel<FAT_CHECK_SHARED>), grid, dim3(fat::kRowsThreads), 0, stream, prm);
+      break;
     case FAT_CHECK_COPY:
       hipLaunchKernelGGL((fat::check_lists_kernel<FAT_CHECK_COPY>), grid, dim3(fat::kListThreads), 0, stream, prm);
       break;

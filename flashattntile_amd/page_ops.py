@@ -172,9 +172,7 @@ def copy_pages(cache: PagedKVCache, src: torch.Tensor, dst: torch.Tensor, *, qua
     with _on(dev):
         stream = _hip.current_stream_handle(dev)
         if validate:
-            scratch = torch.empty(cache.num_pages, dtype=torch.int32, device=dev)
-            check = _hip.check_begin(_hip.CHECK_COPY, stream, dev, ids=(src, dst), scratch=scratch,
-                                     num_pages=cache.num_pages)
+            check = _hip.check_begin(_hip.CHECK_COPY, stream, dev, ids=(src, dst), num_pages=cache.num_pages)
             _copy_flags(check.wait()[7], cache)
         _hip.copy_pages(cache, src, dst, copy, scales, stream)
 
@@ -213,10 +211,9 @@ def fork_sequences(cache: PagedKVCache, parents: torch.Tensor, children: torch.T
     with _on(dev):
         stream = _hip.current_stream_handle(dev)
         if validate:
-            scratch = torch.empty(cache.num_pages + cache.batch_size, dtype=torch.int32, device=dev)
             check = _hip.check_begin(_hip.CHECK_FORK, stream, dev, seq_lens=cache.seq_lens,
                                      page_table=cache.page_table, page_size=cache.page_size,
-                                     ids=(parents, children, pages), scratch=scratch, num_pages=cache.num_pages)
+                                     ids=(parents, children, pages), num_pages=cache.num_pages)
             _fork_flags(check.wait()[7], cache)
         _hip.fork_sequences(cache, parents, children, pages, copy, scales, stream)
 

@@ -46,7 +46,8 @@
 extern "C" {
 #endif
 
-/* 19: fat_paged_decode_shared and FAT_CHECK_SHARED.
+/* 20: FAT_CHECK_COPY and FAT_CHECK_FORK need no scratch memory.
+ * 19: fat_paged_decode_shared and FAT_CHECK_SHARED.
  * 18: operations on pages (fat_copy_pages, fat_fork_sequences,
  *     fat_free_sequences, fat_compact_pages) and FAT_CHECK_COPY, _FORK, _FREE.
  * 17: fat_decode_args.workspace_bytes; fat_stream_capture_id.
@@ -71,7 +72,7 @@ extern "C" {
  * 8: fp32 decode, any page size and head_dim 32/256 through the generic
  *    decode kernel (FAT_KERNEL_DECODE_GENERIC); the paged prefill `rows`
  *    field replaces the library's environment overrides. */
-#define FAT_ABI_VERSION 19
+#define FAT_ABI_VERSION 20
 
 /* Element types understood by the kernels. */
 enum fat_dtype {
@@ -766,9 +767,7 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *          prefix (of a group with sequences); 8 the most keys behind the prefix;
  *          9 sum over groups of prefix; 10 sum over sequences of the keys behind
  *          it; 11 sum over groups of prefix x sequences
- * Entries that a kind doesn't name are undefined.  `scratch` (COPY: int32
- * [num_pages], FORK: int32 [num_pages + batch], device memory) need not be
- * cleared and holds nothing afterwards.
+ * Entries that a kind doesn't name are undefined.
  */
 enum fat_check_kind {
   FAT_CHECK_CACHE = 0,
@@ -798,8 +797,7 @@ typedef struct fat_check_args {
   int32_t page_size;
   const float* values; /* [count], RANGE only */
   int64_t count;
-  const int32_t* ids[3]; /* [count] each: COPY, FORK and FREE only */
-  int32_t* scratch;
+  const int32_t* ids[3]; /* [count] each: COPY, FORK, FREE and SHARED only */
   int32_t num_pages; /* COPY and FORK only */
   int32_t tokens;    /* SHARED only */
 } fat_check_args;
