@@ -12,6 +12,7 @@ kernels are enqueued on torch's current HIP stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import struct
@@ -570,6 +571,14 @@ def lib() -> ctypes.CDLL:
     if _LIB is None:
         raise RuntimeError(f"HIP kernel library unavailable: {_ERROR}")
     return _LIB
+
+
+def on_device(device: torch.device):
+    """Make ``device`` the current one, where it isn't (the launches and a
+    check's page-locked words belong to it)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 class Check:

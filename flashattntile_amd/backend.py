@@ -9,12 +9,14 @@ metadata fields and errors):
 * ``forward(query, kv_cache, attn_metadata)`` runs causal varlen prefill when
   ``attn_metadata.is_prefill`` and paged decode otherwise.
 
-Two extension fields the reference backend lacks:
+Extension fields the reference backend lacks:
 * ``kv_scales``: an int8/fp8 :class:`PagedKVCache` is routed to the quantised
   decode kernel when it carries the cache's scales;
 * ``paged_prefill``: prefill reads K/V from ``kv_cache`` through the page
   table (chunked prefill; the chunk's own K/V already appended) instead of
-  from the packed ``k``/``v`` the reference requires (``backend.py:158-162``).
+  from the packed ``k``/``v`` the reference requires (``backend.py:158-162``);
+* ``cu_groups`` and ``prefix_lens``: decode of groups of sequences that share
+  a prefix, whose keys are read once per group;
 
 and one extension of the decode route: a ``[batch, q_len, heads, head_dim]``
 query with ``q_len > 1`` (speculative verification, the tokens' K/V already
@@ -30,6 +32,7 @@ import torch
 
 from .kernels.decode import paged_decode_attention, paged_decode_attention_fp8, paged_decode_attention_multi
 from .kernels.prefill import paged_prefill_attention, prefill_attention
+from .kernels.shared import paged_decode_attention_shared
 from .paging import PagedKVCache, allocate
 
 
@@ -52,6 +55,9 @@ class AttentionMetadata:
     kv_scales: object | None = None
     # Prefill from the paged cache (chunk K/V already appended) instead of k/v.
     paged_prefill: bool = False
+    # Decode: sequences cu_groups[g] .. cu_groups[g + 1] - 1 share their first prefix_lens[g] keys.
+    cu_groups: torch.Tensor | None = None
+    prefix_lens: torch.Tensor | None = None
 
 
 def get_kv_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int,
@@ -75,7 +81,7 @@ class FlashAttnTileBackend:
     behind the wrappers of :mod:`flashattntile_amd.kernels`.
     """
 
-    ROUTES = ("decode", "decode_quant", "decode_multi", "prefill", "prefill_paged")
+    ROUTES = ("decode", "decode_quant", "decode_multi", "decode_shared", "prefill", "prefill_paged")
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                  dtype: torch.dtype | None = None, device: torch.device | str | None = None) -> None:
@@ -115,6 +121,8 @@ class FlashAttnTileBackend:
 
         * prefill metadata -> ``prefill`` (packed K/V, ``backend.py:155-173``)
           or ``prefill_paged`` (K/V read through the page table);
+        * decode with ``cu_groups`` -> ``decode_shared``, for 3-D and 4-D
+          queries and 8-bit caches too;
         * decode with a ``[batch, q_len > 1, heads, head_dim]`` query ->
           ``decode_multi``;
         * other decode calls -> ``decode_quant`` when the metadata carries
@@ -123,6 +131,8 @@ class FlashAttnTileBackend:
         meta = attn_metadata
         if meta.is_prefill:
             return "prefill_paged" if meta.paged_prefill else "prefill"
+        if meta.cu_groups is not None:
+            return "decode_shared"
         if query.dim() == 4 and query.shape[1] > 1:
             return "decode_multi"
         return "decode" if meta.kv_scales is None else "decode_quant"
@@ -154,6 +164,16 @@ class FlashAttnTileBackend:
         cache = self._with_metadata(kv_cache, meta)
         way = self.route(query, meta)
         scale = meta.softmax_scale
+        if way == "decode_shared":
+            if meta.prefix_lens is None:
+                raise ValueError("shared-prefix decode routing requires prefix_lens with cu_groups")
+            if query.dim() == 4 and query.shape[1] == 1:
+                query = query.squeeze(1)
+            if query.dim() not in (3, 4):
+                raise ValueError(f"query must be 3-D or 4-D, got {tuple(query.shape)}")
+            self._check_heads(query.shape[-2])
+            return paged_decode_attention_shared(query, cache, meta.cu_groups, meta.prefix_lens, softmax_scale=scale,
+                                                 scales=meta.kv_scales)
         if way == "decode_multi":
             self._check_heads(query.shape[2])
             return paged_decode_attention_multi(query, cache, softmax_scale=scale, scales=meta.kv_scales)

@@ -186,9 +186,11 @@ def paged_decode_shared_launch(q: torch.Tensor, cache: PagedKVCache, cu_groups: 
     x partials x (head_dim + 2) bytes) may be passed in to avoid allocations.
     Takes fp16/bf16 queries at head_dim 64 or 128, else raises.
     """
-    a, out, _keep = _block(q, cache, cu_groups, prefix_lens, softmax_scale, scales, out)
-    cfg = _resolve(config, q, cache, max_prefix, max_own, max_group or q.shape[0], prefix_lens.shape[0], q.shape[0])
-    _launch(a, q, cfg, max_group or q.shape[0], workspace)
+    with _hip.on_device(q.device):
+        a, out, _keep = _block(q, cache, cu_groups, prefix_lens, softmax_scale, scales, out)
+        cfg = _resolve(config, q, cache, max_prefix, max_own, max_group or q.shape[0], prefix_lens.shape[0],
+                       q.shape[0])
+        _launch(a, q, cfg, max_group or q.shape[0], workspace)
     return out
 
 
@@ -248,8 +250,8 @@ def paged_decode_attention_shared(
 
     Shapes that the kernel isn't built for (fp32, other head_dims than 64 and
     128, rows that aren't 16-byte aligned) run as ordinary decode, which reads
-    the prefix once per sequence, and so do batches without
-    ``scales`` in which no two sequences share a key.  Returns ``q``'s shape and dtype.
+    the prefix once per sequence, and so do batches without ``scales`` in which no
+    two sequences share a key.  Returns ``q``'s shape and dtype.
     """
     _check_inputs(q, cache, cu_groups, prefix_lens, scales)
     _require_rocm(q, cache, "paged_decode_attention_shared")
@@ -260,22 +262,24 @@ def paged_decode_attention_shared(
     scale = _scale_of(q, softmax_scale)
     q = q.contiguous()
     device = q.device
-    stream = _hip.current_stream_handle(device)
-    sl, pt = cache.seq_lens.contiguous(), cache.page_table
-    pt = pt if pt.stride(-1) == 1 else pt.contiguous()
-    check = _hip.check_begin(_hip.CHECK_SHARED, stream, device, cu_q=cu_groups.contiguous(), seq_lens=sl, page_table=pt,
-                             page_size=cache.page_size, ids=(prefix_lens.contiguous(),), tokens=tokens)
-    # prepared while the check kernel runs
-    block = _block(q, cache, cu_groups, prefix_lens, scale, scales) if _takes(q, cache) else None
-    r = check.wait()
-    _assess(r, q, cache)
-    # Nothing is shared: 64 sequences of 4100 keys took 221 us here, 195 as ordinary
-    # decode (which rounds an 8-bit cache's scaled values to bf16, and so isn't taken there).
-    if block is None or (r[9] == r[11] and scales is None and not given):
-        cfg = _resolve_config(None, q, cache, r[1], r[2], q_len=tokens)
-        return _decode(q, cache, scale, cfg, None, None if scales is None else _dense_scales(scales))
-    a, out, keep = block
-    cfg = _resolve(config, q, cache, r[6], r[8], max(1, r[5]), r[9] / max(1, r[6]), r[10] / max(1, r[8]))
-    _launch(a, q, cfg, max(1, r[5]))
-    del keep
-    return out
+    with _hip.on_device(device):
+        stream = _hip.current_stream_handle(device)
+        sl, pt = cache.seq_lens.contiguous(), cache.page_table
+        pt = pt if pt.stride(-1) == 1 else pt.contiguous()
+        check = _hip.check_begin(_hip.CHECK_SHARED, stream, device, cu_q=cu_groups.contiguous(), seq_lens=sl,
+                                 page_table=pt, page_size=cache.page_size, ids=(prefix_lens.contiguous(),),
+                                 tokens=tokens)
+        # prepared while the check kernel runs
+        block = _block(q, cache, cu_groups, prefix_lens, scale, scales) if _takes(q, cache) else None
+        r = check.wait()
+        _assess(r, q, cache)
+        # Nothing is shared: 64 sequences of 4100 keys took 221 us here, 195 as ordinary
+        # decode (which rounds an 8-bit cache's scaled values to bf16, and so isn't taken there).
+        if block is None or (r[9] == r[11] and scales is None and not given):
+            cfg = _resolve_config(None, q, cache, r[1], r[2], q_len=tokens)
+            return _decode(q, cache, scale, cfg, None, None if scales is None else _dense_scales(scales))
+        a, out, keep = block
+        cfg = _resolve(config, q, cache, r[6], r[8], max(1, r[5]), r[9] / max(1, r[6]), r[10] / max(1, r[8]))
+        _launch(a, q, cfg, max(1, r[5]))
+        del keep
+        return out

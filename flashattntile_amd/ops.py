@@ -11,8 +11,9 @@ Same namespace, names and schemas as ``flashattn_tile/ops.py:35-122``:
     SymInt max_seqlen_q, SymInt max_seqlen_k, bool causal,
     float softmax_scale) -> Tensor``
 
-plus three extensions the reference lacks (its quantised decode had no op,
-its prefill needs packed K/V, and its decode takes one query):
+plus four extensions the reference lacks (its quantised decode had no op,
+its prefill needs packed K/V, its decode takes one query and reads every
+sequence's own keys):
 
 ``flashattn_tile::paged_decode_quant``
     ``(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale,
@@ -28,6 +29,12 @@ its prefill needs packed K/V, and its decode takes one query):
     Tensor? k_scale=None, Tensor? v_scale=None) -> Tensor`` -- multi-token
     (speculative) decode, q ``[batch, q_len, heads, head_dim]``; the
     reference's decode takes one query per sequence (``decode.py:548-553``).
+``flashattn_tile::paged_decode_shared``
+    ``(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table,
+    Tensor seq_lens, Tensor cu_groups, Tensor prefix_lens, SymInt page_size,
+    float softmax_scale, Tensor? k_scale=None, Tensor? v_scale=None) ->
+    Tensor`` -- decode of groups of sequences that share a prefix, q 3-D or,
+    multi-token, 4-D.
 
 The real implementations call the gfx950 HIP kernels through the C ABI; the
 fake implementations touch metadata only, so ``torch.compile(fullgraph=True)``
@@ -40,6 +47,7 @@ import torch
 
 from .kernels.decode import paged_decode_attention, paged_decode_attention_fp8, paged_decode_attention_multi
 from .kernels.prefill import paged_prefill_attention, prefill_attention
+from .kernels.shared import paged_decode_attention_shared
 from .paging import PagedKVCache
 
 __all__ = [
@@ -48,12 +56,14 @@ __all__ = [
     "paged_decode_quant",
     "prefill_paged",
     "paged_decode_multi",
+    "paged_decode_shared",
     "ops_available",
     "PAGED_DECODE_OP",
     "PREFILL_OP",
     "PAGED_DECODE_QUANT_OP",
     "PREFILL_PAGED_OP",
     "PAGED_DECODE_MULTI_OP",
+    "PAGED_DECODE_SHARED_OP",
 ]
 
 PAGED_DECODE_OP = "flashattn_tile::paged_decode"
@@ -61,6 +71,7 @@ PREFILL_OP = "flashattn_tile::prefill_varlen"
 PAGED_DECODE_QUANT_OP = "flashattn_tile::paged_decode_quant"
 PREFILL_PAGED_OP = "flashattn_tile::prefill_paged"
 PAGED_DECODE_MULTI_OP = "flashattn_tile::paged_decode_multi"
+PAGED_DECODE_SHARED_OP = "flashattn_tile::paged_decode_shared"
 
 
 @torch.library.custom_op(PAGED_DECODE_OP, mutates_args=())
@@ -213,8 +224,44 @@ def _paged_decode_multi_fake(q, k_cache, v_cache, page_table, seq_lens, page_siz
     return q.new_empty(q.shape)
 
 
+@torch.library.custom_op(PAGED_DECODE_SHARED_OP, mutates_args=())
+def paged_decode_shared(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_groups: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    page_size: int,
+    softmax_scale: float,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Decode of groups of sequences whose first ``prefix_lens[g]`` keys are the
+    same pages, read once per group.  ``k_scale`` / ``v_scale`` select an int8 /
+    float8_e4m3fn cache."""
+    cache = PagedKVCache(k_cache=k_cache, v_cache=v_cache, page_table=page_table,
+                         seq_lens=seq_lens, page_size=int(page_size))
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("k_scale and v_scale must be given together")
+    scales = None if k_scale is None else {"k": k_scale, "v": v_scale}
+    return paged_decode_attention_shared(q, cache, cu_groups, prefix_lens, softmax_scale=softmax_scale, scales=scales)
+
+
+@paged_decode_shared.register_fake
+def _paged_decode_shared_fake(q, k_cache, v_cache, page_table, seq_lens, cu_groups, prefix_lens, page_size,
+                              softmax_scale, k_scale=None, v_scale=None):
+    torch._check(q.dim() in (3, 4), lambda: f"q must be 3-D or 4-D, got {q.dim()}")
+    torch._check(q.shape[0] == seq_lens.shape[0], lambda: "q batch must match seq_lens")
+    torch._check(q.shape[-1] == k_cache.shape[3], lambda: "q head_dim must match cache")
+    torch._check(q.shape[-2] % k_cache.shape[2] == 0, lambda: "heads must be divisible by KV heads")
+    torch._check(cu_groups.shape[0] == prefix_lens.shape[0] + 1, lambda: "cu_groups must have groups + 1 entries")
+    return q.new_empty(q.shape)
+
+
 def ops_available() -> bool:
     """True when the custom ops are registered in this process."""
     return all(hasattr(torch.ops.flashattn_tile, name)
                for name in ("paged_decode", "prefill_varlen", "paged_decode_quant", "prefill_paged",
-                            "paged_decode_multi"))
+                            "paged_decode_multi", "paged_decode_shared"))

@@ -30,7 +30,6 @@ other checks do, before anything is changed.
 
 from __future__ import annotations
 
-import contextlib
 
 import torch
 
@@ -102,14 +101,6 @@ def _check_rocm(cache: PagedKVCache) -> None:
     _require(cache.seq_lens.is_contiguous(), "seq_lens must be contiguous")
 
 
-def _on(device: torch.device):
-    """Make ``device`` the current one, where it isn't (the launches and the
-    check's page-locked words belong to it)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
 def _copy_flags(flags: int, cache: PagedKVCache) -> None:
     _require(not flags & 1, f"src holds a page outside [0, {cache.num_pages})")
     _require(not flags & 2, f"dst holds a page outside [0, {cache.num_pages})")
@@ -169,7 +160,7 @@ def copy_pages(cache: PagedKVCache, src: torch.Tensor, dst: torch.Tensor, *, qua
 
     dev = cache.k_cache.device
     _require(cache.k_cache.stride(3) == 1 and cache.v_cache.stride(3) == 1, "the head_dim axis must be contiguous")
-    with _on(dev):
+    with _hip.on_device(dev):
         stream = _hip.current_stream_handle(dev)
         if validate:
             check = _hip.check_begin(_hip.CHECK_COPY, stream, dev, ids=(src, dst), num_pages=cache.num_pages)
@@ -208,7 +199,7 @@ def fork_sequences(cache: PagedKVCache, parents: torch.Tensor, children: torch.T
 
     _check_rocm(cache)
     dev = cache.k_cache.device
-    with _on(dev):
+    with _hip.on_device(dev):
         stream = _hip.current_stream_handle(dev)
         if validate:
             check = _hip.check_begin(_hip.CHECK_FORK, stream, dev, seq_lens=cache.seq_lens,
@@ -285,7 +276,7 @@ def free_sequences(cache: PagedKVCache, rows: torch.Tensor, *, held: torch.Tenso
     from . import _hip
 
     _check_rocm(cache)
-    with _on(dev):
+    with _hip.on_device(dev):
         stream = _hip.current_stream_handle(dev)
         check = None
         if validate:
@@ -346,7 +337,7 @@ def compact_pages(cache: PagedKVCache, *, held: torch.Tensor | None = None, quan
     from . import _hip
 
     _check_rocm(cache)
-    with _on(dev):
+    with _hip.on_device(dev):
         stream = _hip.current_stream_handle(dev)
         check = None
         if validate:

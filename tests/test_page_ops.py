@@ -678,3 +678,87 @@ def test_validated_page_operations_are_refused_under_capture():
             compact_pages(cache)
     torch.cuda.synchronize()
     assert torch.equal(cache.page_table, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("P,hkv,d", [(5, 4, 128), (1, 4, 128), (11, 4, 128), (8, 1, 64), (32, 4, 64), (100, 2, 256)])
+@pytest.mark.parametrize("pairs", [1, 2, 7, 65])
+def test_copy_of_pages_of_whole_chunks(P, hkv, d, pairs):
+    """Pages of 1, 5, 11, 16 and 100 KiB: a wave's eight chunks begin and end anywhere in them."""
+    print(f"chunks {P} {hkv} {d} {pairs}", flush=True)
+    cache = _cache([1], P, hkv, d, torch.float16, "cuda", spare=2 * pairs + 3, seed=pairs)
+    order = torch.randperm(cache.num_pages, generator=torch.Generator().manual_seed(pairs)).tolist()
+    src, dst = order[:pairs], order[pairs:2 * pairs]
+    before = _snapshot(cache)
+    copy_pages(cache, _ids(src, "cuda"), _ids(dst, "cuda"))
+    _same(_snapshot(cache), _moved(before, list(zip(src, dst))))
+
+
+def _huge(pages, rows=3, width=4, P=1):
+    """A pool of many tiny pages."""
+    k = torch.arange(pages * 2, dtype=torch.int32, device="cuda").view(pages, P, 1, 2).to(torch.float32)
+    table = torch.zeros(rows, width, dtype=torch.int32, device="cuda")
+    return PagedKVCache(k, -k, table, _ids([0] * rows, "cuda"), P)
+
+
+@pytest.mark.gpu
+def test_ids_of_pools_that_take_several_turns_of_the_bitmap():
+    """Repetitions and overlaps on both sides of every 2^19 ids."""
+    turn = 1 << 19
+    pages = 2 * turn + 100
+    cache = _huge(pages)
+    print("several turns", flush=True)
+    src = [0, turn - 1, turn + 1, 2 * turn + 99, turn - 1]
+    dst = [turn, 2 * turn, 5, 2 * turn - 1, 7]
+    before = _snapshot(cache)
+    copy_pages(cache, _ids(src, "cuda"), _ids(dst, "cuda"))
+    _same(_snapshot(cache), _moved(before, list(zip(src, dst))))
+    for bad, error in ((turn, "twice"), (2 * turn, "twice"), (turn - 1, "src holds too"), (turn + 1, "src holds too"),
+                       (2 * turn + 99, "src holds too"), (pages, "dst holds a page outside"), (-1, "dst holds a page")):
+        with pytest.raises(AssertionError, match=error):
+            copy_pages(cache, _ids(src, "cuda"), _ids(dst[:4] + [bad], "cuda"))
+    cache.page_table.copy_(_ids([[2 * turn + 98, 0, 0, 0], [turn + 3, 9, 0, 0], [0, 0, 0, 0]], "cuda"))
+    cache = PagedKVCache(cache.k_cache.view(pages // 2, 2, 1, 2), cache.v_cache.view(pages // 2, 2, 1, 2),
+                         torch.zeros(4, 2, dtype=torch.int32, device="cuda"), _ids([1, 1, 0, 0], "cuda"), 2)
+    cache.page_table[0, 0], cache.page_table[1, 0] = pages // 2 - 1, 3
+    for take in ([turn, turn], [pages // 2 - 7] * 2):
+        with pytest.raises(AssertionError, match="pages holds a page twice"):
+            fork_sequences(cache, _ids([0, 1], "cuda"), _ids([2, 3], "cuda"), _ids(take, "cuda"))
+    fork_sequences(cache, _ids([0, 1], "cuda"), _ids([2, 3], "cuda"), _ids([turn, 0], "cuda"))
+    assert cache.page_table[2:, 0].tolist() == [turn, 0] and cache.seq_lens.tolist() == [1, 1, 1, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages,rows,width", [(65536, 4, 8192), (65537, 4, 8192), (65536, 4, 8193), (70, 1, 32768),
+                                              (70, 32768, 1), (70, 17, 5), (200, 33, 3)])
+def test_free_and_compact_where_one_workgroup_ends(pages, rows, width):
+    """Pools and tables at the largest that one workgroup lists, and one beyond."""
+    print(f"one workgroup {pages} {rows} {width}", flush=True)
+    g = torch.Generator().manual_seed(pages + width)
+    cache = _huge(pages, rows, width)
+    table = torch.randint(0, pages, (rows, width), generator=g, dtype=torch.int32)
+    lens = torch.randint(0, width + 1, (rows,), generator=g, dtype=torch.int32)
+    cache.page_table.copy_(table)
+    cache.seq_lens.copy_(lens)
+    gone = sorted({0, rows // 2, rows - 1}) if rows > 1 else []
+    got, count = free_sequences(cache, _ids(gone, "cuda"))
+    lens[gone] = 0
+    assert torch.equal(cache.seq_lens.cpu(), lens)
+    used = torch.zeros(pages, dtype=torch.bool)
+    seen = torch.arange(width)[None] < lens[:, None]
+    used[table[seen].long()] = True
+    free = (~used).nonzero()[:, 0].to(torch.int32)
+    assert int(count) == len(free) and torch.equal(got[:len(free)].cpu(), free)
+    assert bool((got[len(free):] == -1).all())
+    before = _snapshot(cache)
+    remap, n = compact_pages(cache)
+    n = int(n)
+    assert n == int(used.sum())
+    ids = torch.arange(pages)
+    src, dst = ids[used & (ids >= n)], ids[~used & (ids < n)]
+    want = torch.where(used, ids, torch.full_like(ids, -1))
+    want[src] = dst
+    assert torch.equal(remap.cpu().long(), want)
+    _same(_snapshot(cache), _moved(before, list(zip(src.tolist(), dst.tolist()))))
+    table[seen] = want[table[seen].long()].to(torch.int32)
+    assert torch.equal(cache.page_table.cpu(), table)
