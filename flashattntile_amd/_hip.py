@@ -610,8 +610,8 @@ class Check:
         a = self._args
         a.kind = kind
         a.batch = batch
+        a.count = ids[0].numel() if ids else 0
         if ids:
-            a.count = ids[0].numel()
             for i, t in enumerate(ids):
                 a.ids[i] = t.data_ptr()
             a.num_pages = num_pages
@@ -1147,44 +1147,45 @@ def _set_pool(a: Pool, cache, quantized=None, scales=None) -> None:
     """Fill ``a`` with the pages of ``cache``, its 8-bit copy ``quantized`` (K
     and V pages, K and V scales) or, for an 8-bit cache, its ``scales``."""
     k, v = cache.k_cache, cache.v_cache
-    a.k_cache, a.v_cache = _ptr(k), _ptr(v)
-    a.k_stride_page, a.k_stride_slot, a.k_stride_head = k.stride(0), k.stride(1), k.stride(2)
-    a.v_stride_page, a.v_stride_slot, a.v_stride_head = v.stride(0), v.stride(1), v.stride(2)
+    a.k_cache, a.v_cache = k.data_ptr(), v.data_ptr()
+    a.k_stride_page, a.k_stride_slot, a.k_stride_head, _ = k.stride()
+    a.v_stride_page, a.v_stride_slot, a.v_stride_head, _ = v.stride()
     if quantized is not None:
         qk, qv, *scales = quantized
-        a.quant_k_cache, a.quant_v_cache = _ptr(qk), _ptr(qv)
-        a.qk_stride_page, a.qk_stride_slot, a.qk_stride_head = qk.stride(0), qk.stride(1), qk.stride(2)
-        a.qv_stride_page, a.qv_stride_slot, a.qv_stride_head = qv.stride(0), qv.stride(1), qv.stride(2)
+        a.quant_k_cache, a.quant_v_cache = qk.data_ptr(), qv.data_ptr()
+        a.qk_stride_page, a.qk_stride_slot, a.qk_stride_head, _ = qk.stride()
+        a.qv_stride_page, a.qv_stride_slot, a.qv_stride_head, _ = qv.stride()
     if scales is not None:
-        a.k_scale, a.v_scale = _ptr(scales[0]), _ptr(scales[1])
-        a.scale_stride_page, a.scale_stride_head = scales[0].stride(0), scales[0].stride(1)
+        a.k_scale, a.v_scale = scales[0].data_ptr(), scales[1].data_ptr()
+        a.scale_stride_page, a.scale_stride_head = scales[0].stride()
     a.num_pages, a.page_size, a.num_kv_heads, a.head_dim = k.shape
     a.dtype = dtype_code(k.dtype)
 
 
 def _set_table(a, cache) -> None:
-    a.page_table, a.seq_lens = _ptr(cache.page_table), _ptr(cache.seq_lens)
+    a.page_table, a.seq_lens = cache.page_table.data_ptr(), cache.seq_lens.data_ptr()
     a.page_table_stride = cache.page_table.stride(0)
     a.batch, a.max_pages = cache.page_table.shape
 
 
-def copy_pages(cache, src: torch.Tensor, dst: torch.Tensor, quantized, scales, stream: int) -> None:
-    """Enqueue ``fat_copy_pages`` of already-validated device tensors
+def copy_pages_args(cache, src: torch.Tensor, dst: torch.Tensor, quantized, scales) -> CopyPagesArgs:
+    """``fat_copy_pages_args`` of already-validated device tensors
     (``quantized`` and ``scales`` as :func:`_set_pool` takes them)."""
     a = CopyPagesArgs()
     _set_pool(a.pool, cache, quantized, scales)
-    a.src, a.dst, a.count = _ptr(src), _ptr(dst), src.numel()
-    _check(lib().fat_copy_pages(ctypes.byref(a), _c_vp(stream)), "fat_copy_pages")
+    a.src, a.dst, a.count = src.data_ptr(), dst.data_ptr(), src.numel()
+    return a
 
 
-def fork_sequences(cache, parents: torch.Tensor, children: torch.Tensor, pages: torch.Tensor, quantized, scales,
-                   stream: int) -> None:
-    """Enqueue ``fat_fork_sequences``."""
+def fork_args(cache, parents: torch.Tensor, children: torch.Tensor, pages: torch.Tensor, quantized,
+              scales) -> ForkArgs:
+    """``fat_fork_args``."""
     a = ForkArgs()
     _set_pool(a.pool, cache, quantized, scales)
     _set_table(a, cache)
-    a.parents, a.children, a.pages, a.count = _ptr(parents), _ptr(children), _ptr(pages), parents.numel()
-    _check(lib().fat_fork_sequences(ctypes.byref(a), _c_vp(stream)), "fat_fork_sequences")
+    a.parents, a.children, a.pages = parents.data_ptr(), children.data_ptr(), pages.data_ptr()
+    a.count = parents.numel()
+    return a
 
 
 def pages_workspace(num_pages: int, device: torch.device) -> torch.Tensor:
@@ -1192,22 +1193,28 @@ def pages_workspace(num_pages: int, device: torch.device) -> torch.Tensor:
     return torch.empty(int(lib().fat_pages_workspace_bytes(num_pages)), dtype=torch.uint8, device=device)
 
 
-def free_sequences(cache, rows: torch.Tensor, held: torch.Tensor | None, pages: torch.Tensor, num_free: torch.Tensor,
-                   workspace: torch.Tensor, stream: int) -> None:
-    """Enqueue ``fat_free_sequences``."""
+def free_args(cache, rows: torch.Tensor, held: torch.Tensor | None, pages: torch.Tensor, num_free: torch.Tensor,
+              workspace: torch.Tensor) -> FreeArgs:
+    """``fat_free_args``."""
     a = FreeArgs()
     _set_table(a, cache)
-    a.held, a.rows, a.pages, a.num_free = _ptr(held), _ptr(rows), _ptr(pages), _ptr(num_free)
-    a.workspace = _ptr(workspace)
+    a.held, a.rows, a.pages, a.num_free = _ptr(held), _ptr(rows), pages.data_ptr(), num_free.data_ptr()
+    a.workspace = workspace.data_ptr()
     a.num_pages, a.page_size, a.count = cache.k_cache.shape[0], cache.page_size, rows.numel()
-    _check(lib().fat_free_sequences(ctypes.byref(a), _c_vp(stream)), "fat_free_sequences")
+    return a
 
 
-def compact_pages(cache, held: torch.Tensor | None, remap: torch.Tensor, num_used: torch.Tensor,
-                  workspace: torch.Tensor, quantized, scales, stream: int) -> None:
-    """Enqueue ``fat_compact_pages``."""
+def compact_args(cache, held: torch.Tensor | None, remap: torch.Tensor, num_used: torch.Tensor,
+                 workspace: torch.Tensor, quantized, scales) -> CompactArgs:
+    """``fat_compact_args``."""
     a = CompactArgs()
     _set_pool(a.pool, cache, quantized, scales)
     _set_table(a, cache)
-    a.held, a.remap, a.num_used, a.workspace = _ptr(held), _ptr(remap), _ptr(num_used), _ptr(workspace)
-    _check(lib().fat_compact_pages(ctypes.byref(a), _c_vp(stream)), "fat_compact_pages")
+    a.held, a.remap, a.num_used, a.workspace = _ptr(held), remap.data_ptr(), num_used.data_ptr(), workspace.data_ptr()
+    return a
+
+
+def page_operation(name: str, a, stream: int) -> None:
+    """Enqueue ``fat_copy_pages``, ``fat_fork_sequences``, ``fat_free_sequences``
+    or ``fat_compact_pages`` with a prepared argument block."""
+    _check(getattr(lib(), name)(ctypes.byref(a), _c_vp(stream)), name)

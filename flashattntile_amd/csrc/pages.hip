@@ -59,7 +59,11 @@ __device__ __forceinline__ int64_t divide(int64_t x, uint32_t by, uint32_t& rest
 // Pages that are runs of 1 KiB chunks (all but slices of a pool, and scales):
 // 32 chunks of them, 8 per wave.  A chunk has one pair of ids, so its addresses
 // are scalar, and a lane holds nothing but its 16 bytes of each chunk: all of a
-// wave's loads are in flight before its first store, at full occupancy.
+// wave's loads are in flight before its first store, at full occupancy.  Copying
+// 12000 scattered pages of 32 KiB reaches 4.9 TB/s (read and written), pages in a
+// row 5.5, torch's copy of such a tensor 5.1; with an address per lane and 128
+// registers a thread it was 3.6.  Plain stores: past the caches they gain 2 % where
+// the pool is larger than those and lose 20 % where it isn't.
 template <typename Pair>
 __device__ __forceinline__ void copy_chunks(const Plane& pl, int64_t step, int64_t count, Pair pair) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -74,7 +78,8 @@ __device__ __forceinline__ void copy_chunks(const Plane& pl, int64_t step, int64
   for (int u = 0; u < kWaveChunks; ++u) {
     to[u] = nullptr;
     if (on) {
-      x[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(pl.base + (int64_t)s * pl.page + (int64_t)c * kChunk + lane));
+      const uint8_t* from = pl.base + (int64_t)s * pl.page + (int64_t)c * kChunk;
+      x[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + lane));
       to[u] = pl.base + (int64_t)d * pl.page + (int64_t)c * kChunk;
     }
     if (++c == pl.cpp) {
@@ -138,9 +143,8 @@ __device__ __forceinline__ void copy_step(const Plane& pl, int64_t step, int64_t
 
 // blockIdx.y: plane; blockIdx.x: steps of it, the grid's width apart.
 __global__ __launch_bounds__(kCopyThreads, 8) void copy_pages_kernel(const Planes planes,
-                                                                                  const int32_t* __restrict__ src,
-                                                                                  const int32_t* __restrict__ dst,
-                                                                                  int64_t count) {
+                                                                     const int32_t* __restrict__ src,
+                                                                     const int32_t* __restrict__ dst, int64_t count) {
   const Plane pl = planes.p[blockIdx.y];
   const int64_t steps = plane_steps(pl, count);
   for (int64_t step = blockIdx.x; step < steps; step += gridDim.x)
@@ -165,6 +169,8 @@ struct ForkParams {
   int32_t B, max_pages, P;
 };
 
+// 240 forks of pages of 384 KiB (with their 8-bit copy) take 39 us: 92 MB written,
+// 2.4 TB/s, as a copy's writes.
 // blockIdx.y: the fork; blockIdx.z: a plane of its last page, or (the last) its
 // table row; blockIdx.x: steps.  Every workgroup of a fork reads only its
 // parent's row, which no fork of the call writes, and decides alike.
@@ -250,14 +256,18 @@ __global__ __launch_bounds__(kUseThreads) void use_clear_kernel(const UseParams 
   }
 }
 
-// blockIdx.y: rows, the grid's height apart; blockIdx.x: 1024 columns.
+// blockIdx.y: rows, the grid's height apart; blockIdx.x: 4096 columns.  Bound by
+// the scattered byte stores, whose lines every XCD's L2 writes back: 14 us for 1.1
+// million ids, 4 of them for reading those (17 at 1024 columns; 27 and 35 with
+// stores that go past the L2).
+constexpr int kMarkEach = 16;  // columns per thread
 __global__ __launch_bounds__(kUseThreads) void use_mark_kernel(const UseParams p) {
   for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
     const int n = used_columns(p, b);
     const int32_t* row = p.pt + (int64_t)b * p.pt_sb;
-    const int c0 = blockIdx.x * (4 * kUseThreads) + threadIdx.x;
+    const int c0 = blockIdx.x * (kMarkEach * kUseThreads) + threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kMarkEach; ++u) {
       const int c = c0 + u * kUseThreads;
       if (c < n) {
         const int id = row[c];
@@ -298,24 +308,37 @@ __global__ __launch_bounds__(kUseThreads) void use_count_kernel(const UseParams 
   if (threadIdx.x == 0) p.counts[blockIdx.x] = n;
 }
 
-// Writes the lists: a thread has 16 ids.  COMPACT: sources and destinations of
-// the moves and the new ids of the pages that stay, else the free pages.
+// Writes the lists.  COMPACT: sources and destinations of the moves and the new
+// ids of the pages that stay, else the free pages.  A wave has 64 ids at a time,
+// whose flags are a ballot, so that its stores lie next to each other (a thread
+// with 16 ids in a row took 9.7 instead of 5 us for 1.4 million ids).
 template <bool COMPACT>
 __global__ __launch_bounds__(kUseThreads) void use_list_kernel(const UseParams p) {
+  constexpr int kWaves = kUseThreads / 64, kEach = kUseGroup / kUseThreads;
+  __shared__ int s_before[kEach * kWaves];
   const int groups = gridDim.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int mine = 0, all = 0, dummy;
   for (int i = threadIdx.x; i < groups; i += kUseThreads) {
     const int c = p.counts[i];
     all += c;
     mine += i < (int)blockIdx.x ? c : 0;
   }
-  const int n = use_scan(all, dummy);
+  unsigned long long flags[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    flags[j] = __ballot(p.used[(int64_t)blockIdx.x * kUseGroup + j * kUseThreads + threadIdx.x] != 0);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (lane == 0) s_before[j * kWaves + wave] = __popcll(flags[j]);
+  }
+  const int n = use_scan(all, dummy);  // (synchronises)
   const int first = use_scan(mine, dummy);
-  u32x4 f = reinterpret_cast<const u32x4*>(p.used)[(int64_t)blockIdx.x * kUseThreads + threadIdx.x];
-  int rank;  // used ids before this thread's
-  use_scan(__popc(f[0]) + __popc(f[1]) + __popc(f[2]) + __popc(f[3]), rank);
-  rank += first;
-  const int id0 = blockIdx.x * kUseGroup + threadIdx.x * 16;
+  int before = 0, x = wave == 0 ? s_before[lane] : 0;
+  static_assert(kEach * kWaves == 64, "a wave scans the counts of a group's 64 ids each");
+  use_scan(x, before);
+  if (wave == 0) s_before[lane] = first + before;
+  __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.total = COMPACT ? n : p.num_pages - n;
   // COMPACT: used ids below n, from whom the moved ones' ranks count.  They are
   // the used ids of the whole groups below n and those of its own group.
@@ -324,38 +347,34 @@ __global__ __launch_bounds__(kUseThreads) void use_list_kernel(const UseParams p
     const int gn = n / kUseGroup;
     int w = 0;
     for (int i = threadIdx.x; i < min(gn, groups); i += kUseThreads) w += p.counts[i];
-    below = use_scan(w, dummy);
     if (gn < groups) {
       const u32x4 h = reinterpret_cast<const u32x4*>(p.used)[(int64_t)gn * kUseThreads + threadIdx.x];
       const int k0 = gn * kUseGroup + threadIdx.x * 16;
-      int x = 0;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x += k0 + j < n ? (int)((h[j / 4] >> (8 * (j % 4))) & 1) : 0;
-      below += use_scan(x, dummy);
+      for (int j = 0; j < 16; ++j) w += k0 + j < n ? (int)((h[j / 4] >> (8 * (j % 4))) & 1) : 0;
     }
+    below = use_scan(w, dummy);
   }
   const int nfree = p.num_pages - n;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int id = id0 + j;
-    const bool used = (f[j / 4] >> (8 * (j % 4))) & 1;
+  for (int j = 0; j < kEach; ++j) {
+    const int id = blockIdx.x * kUseGroup + j * kUseThreads + threadIdx.x;
+    const bool used = (flags[j] >> lane) & 1;
+    const int rank = s_before[j * kWaves + wave] + __popcll(flags[j] & ((1ull << lane) - 1));
     if (id < p.num_pages) {
       if constexpr (COMPACT) {
-        int to = -1;
-        if (used && id < n) to = id;
         if (!used && id < n) p.list[id - rank] = id;
         if (used && id >= n) {
           p.src[rank - below] = id;
           p.rank[id] = rank - below;
         } else {
-          p.remap[id] = to;
+          p.remap[id] = used ? id : -1;
         }
       } else {
         if (!used) p.list[id - rank] = id;
         else p.list[nfree + rank] = -1;
       }
     }
-    rank += used ? 1 : 0;
   }
   if constexpr (COMPACT) {
     if (blockIdx.x == 0 && threadIdx.x == 0) p.counts[groups] = n - below;  // moves
@@ -434,7 +453,7 @@ __global__ __launch_bounds__(kSmallThreads) void use_small_kernel(const UseParam
 
 // The moves: blockIdx.y < n planes: copies of that plane; the last: new ids.
 __global__ __launch_bounds__(kCopyThreads, 8) void compact_apply_kernel(const Planes planes, const UseParams p,
-                                                                     int groups) {
+                                                                        int groups) {
   const int moves = p.counts[groups];
   if ((int)blockIdx.y < planes.n) {
     const Plane pl = planes.p[blockIdx.y];
@@ -449,7 +468,8 @@ __global__ __launch_bounds__(kCopyThreads, 8) void compact_apply_kernel(const Pl
   }
   const int n = *p.total;
   const int64_t stride = (int64_t)gridDim.x * kCopyThreads;
-  for (int64_t i = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x; i < moves; i += stride) p.remap[p.src[i]] = p.list[i];
+  for (int64_t i = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x; i < moves; i += stride)
+    p.remap[p.src[i]] = p.list[i];
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
     const int cols = used_columns(p, b);
     int32_t* row = p.pt + (int64_t)b * p.pt_sb;
@@ -610,8 +630,8 @@ bool use_args_ok(const void* lens, const void* pt, int64_t pt_sb, int batch, int
     fat_host::set_error("%s: a required pointer is NULL", who);
     return false;
   }
-  if (batch < 0 || max_pages <= 0 || num_pages <= 0 || num_pages > (1 << 30) || P <= 0 || pt_sb < 0 || (batch > 1 && pt_sb < max_pages) ||
-      (uintptr_t)ws % 16) {
+  if (batch < 0 || max_pages <= 0 || num_pages <= 0 || num_pages > (1 << 30) || P <= 0 || pt_sb < 0 ||
+      (batch > 1 && pt_sb < max_pages) || (uintptr_t)ws % 16) {
     fat_host::set_error("%s: batch %d, max_pages %d, num_pages %d, page_size %d, page_table_stride %lld or the "
                         "workspace's alignment invalid", who, batch, max_pages, num_pages, P, (long long)pt_sb);
     return false;
@@ -635,8 +655,8 @@ int launch_use(const fat::UseParams& p, hipStream_t stream) {
   int rc = fat_host::launch_status("use_clear_kernel");
   if (rc != FAT_OK) return rc;
   if (p.B > 0) {
-    const dim3 grid((unsigned)((p.max_pages + 4 * fat::kUseThreads - 1) / (4 * fat::kUseThreads)),
-                    (unsigned)std::min(p.B, 32768));
+    constexpr int kColumns = fat::kMarkEach * fat::kUseThreads;
+    const dim3 grid((unsigned)((p.max_pages + kColumns - 1) / kColumns), (unsigned)std::min(p.B, 32768));
     hipLaunchKernelGGL(fat::use_mark_kernel, grid, dim3(fat::kUseThreads), 0, stream, p);
     if ((rc = fat_host::launch_status("use_mark_kernel")) != FAT_OK) return rc;
   }

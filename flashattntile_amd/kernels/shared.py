@@ -199,7 +199,7 @@ def _resolve(config, q, cache, max_prefix: int, max_own: int, max_group: int, gr
     per_seq = (q.shape[1] if q.dim() == 4 else 1) * q.shape[-2] // cache.num_kv_heads
     cfg = shared_splits(cache.num_kv_heads, max_group * per_seq, -(-per_seq // 32), groups, max_prefix, sequences,
                         max_own)
-    given = _given(config)
+    given = _given(config) if config else None
     if not given:
         return cfg
     row_blocks = given.pop("row_blocks", 0)

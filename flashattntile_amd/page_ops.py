@@ -30,10 +30,9 @@ other checks do, before anything is changed.
 
 from __future__ import annotations
 
-
 import torch
 
-from .paging import PagedKVCache, _assess_cache, _check_layout, _quant_pair, _require, cache_stats
+from .paging import PagedKVCache, _assess_cache, _check_layout, _quant_pair, _require
 
 __all__ = ["copy_pages", "fork_sequences", "free_sequences", "compact_pages"]
 
@@ -162,10 +161,13 @@ def copy_pages(cache: PagedKVCache, src: torch.Tensor, dst: torch.Tensor, *, qua
     _require(cache.k_cache.stride(3) == 1 and cache.v_cache.stride(3) == 1, "the head_dim axis must be contiguous")
     with _hip.on_device(dev):
         stream = _hip.current_stream_handle(dev)
+        check = None
         if validate:
             check = _hip.check_begin(_hip.CHECK_COPY, stream, dev, ids=(src, dst), num_pages=cache.num_pages)
+        args = _hip.copy_pages_args(cache, src, dst, copy, scales)  # prepared while the check kernel runs
+        if check is not None:
             _copy_flags(check.wait()[7], cache)
-        _hip.copy_pages(cache, src, dst, copy, scales, stream)
+        _hip.page_operation("fat_copy_pages", args, stream)
 
 
 def fork_sequences(cache: PagedKVCache, parents: torch.Tensor, children: torch.Tensor, pages: torch.Tensor, *,
@@ -201,12 +203,15 @@ def fork_sequences(cache: PagedKVCache, parents: torch.Tensor, children: torch.T
     dev = cache.k_cache.device
     with _hip.on_device(dev):
         stream = _hip.current_stream_handle(dev)
+        check = None
         if validate:
             check = _hip.check_begin(_hip.CHECK_FORK, stream, dev, seq_lens=cache.seq_lens,
                                      page_table=cache.page_table, page_size=cache.page_size,
                                      ids=(parents, children, pages), num_pages=cache.num_pages)
+        args = _hip.fork_args(cache, parents, children, pages, copy, scales)  # prepared while the check kernel runs
+        if check is not None:
             _fork_flags(check.wait()[7], cache)
-        _hip.fork_sequences(cache, parents, children, pages, copy, scales, stream)
+        _hip.page_operation("fat_fork_sequences", args, stream)
 
 
 def _fork_torch(cache, parents, children, pages, copy, scales) -> None:
@@ -248,6 +253,17 @@ def _used_torch(cache: PagedKVCache, held: torch.Tensor | None) -> tuple[torch.T
     return columns, used
 
 
+def _used_stats(cache: PagedKVCache) -> tuple[int, int, int, int]:
+    """Min and max length, and min and max page id of the columns that each row's
+    tokens use (0, -1 where none does)."""
+    lens = cache.seq_lens.long()
+    if not lens.numel():
+        return 0, 0, 0, -1
+    n = torch.div(lens.clamp_min(0) + cache.page_size - 1, cache.page_size, rounding_mode="floor")
+    ids = cache.page_table[torch.arange(cache.page_table.shape[1], device=n.device) < n[:, None]]
+    return (int(lens.min()), int(lens.max())) + ((int(ids.min()), int(ids.max())) if ids.numel() else (0, -1))
+
+
 def free_sequences(cache: PagedKVCache, rows: torch.Tensor, *, held: torch.Tensor | None = None,
                    validate: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
     """Empty the rows ``rows`` and list the pool's pages that no row uses.
@@ -264,7 +280,7 @@ def free_sequences(cache: PagedKVCache, rows: torch.Tensor, *, held: torch.Tenso
     dev = cache.k_cache.device
     if not cache.k_cache.is_cuda or not cache.page_table.numel() or not cache.num_pages:
         _require(not _outside(rows, cache.batch_size), f"rows holds a row outside [0, {cache.batch_size})")
-        _assess_cache(cache, cache_stats(cache))
+        _assess_cache(cache, _used_stats(cache))
         cache.seq_lens[rows.long()] = 0
         if held is not None:
             held[rows.long()] = 0
@@ -286,17 +302,18 @@ def free_sequences(cache: PagedKVCache, rows: torch.Tensor, *, held: torch.Tenso
         pages = torch.empty(cache.num_pages, dtype=torch.int32, device=dev)
         count = torch.empty((), dtype=torch.int32, device=dev)
         workspace = _hip.pages_workspace(cache.num_pages, dev)
+        args = _hip.free_args(cache, rows, held, pages, count, workspace)
         if check is not None:
             r = check.wait()
             _assess_cache(cache, _stats_of(r))
             _require(not r[7] & 1, f"rows holds a row outside [0, {cache.batch_size})")
-        _hip.free_sequences(cache, rows, held, pages, count, workspace, stream)
+        _hip.page_operation("fat_free_sequences", args, stream)
     return pages, count
 
 
 def _stats_of(r: list[int]) -> tuple[int, int, int, int]:
     """A check's results as :func:`~flashattntile_amd.paging.cache_stats` gives them."""
-    none = r[12] == torch.iinfo(torch.int32).max
+    none = r[12] == 2 ** 31 - 1  # of no used column
     return r[0], r[1], 0 if none else r[12], -1 if none else r[13]
 
 
@@ -321,7 +338,7 @@ def compact_pages(cache: PagedKVCache, *, held: torch.Tensor | None = None, quan
     held = _held(cache, held, written=False)
     dev = cache.k_cache.device
     if not cache.k_cache.is_cuda or not cache.page_table.numel() or not cache.num_pages:
-        _assess_cache(cache, cache_stats(cache))
+        _assess_cache(cache, _used_stats(cache))
         columns, used = _used_torch(cache, held)
         n = int(used.sum())
         ids = torch.arange(cache.num_pages, device=dev)
@@ -341,13 +358,14 @@ def compact_pages(cache: PagedKVCache, *, held: torch.Tensor | None = None, quan
         stream = _hip.current_stream_handle(dev)
         check = None
         if validate:
-            check = _hip.check_begin(_hip.CHECK_CACHE, stream, dev, seq_lens=cache.seq_lens,
+            check = _hip.check_begin(_hip.CHECK_FREE, stream, dev, seq_lens=cache.seq_lens,
                                      page_table=cache.page_table, page_size=cache.page_size)
         # prepared while the check kernel runs
         remap = torch.empty(cache.num_pages, dtype=torch.int32, device=dev)
         count = torch.empty((), dtype=torch.int32, device=dev)
         workspace = _hip.pages_workspace(cache.num_pages, dev)
+        args = _hip.compact_args(cache, held, remap, count, workspace, copy, scales)
         if check is not None:
             _assess_cache(cache, _stats_of(check.wait()))
-        _hip.compact_pages(cache, held, remap, count, workspace, copy, scales, stream)
+        _hip.page_operation("fat_compact_pages", args, stream)
     return remap, count

@@ -731,8 +731,9 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *        FAT_CHECK_COPY    src = ids[0] and dst = ids[1], `count` pages each
  *        FAT_CHECK_FORK    parents, children and pages = ids[0 .. 2], `count`
  *                          each, with seq_lens and the page table
- *        FAT_CHECK_FREE    FAT_CHECK_CACHE, and rows = ids[0], `count` of them
- *        FAT_CHECK_SHARED  FAT_CHECK_CACHE, and the groups cu_q [count + 1] with
+ *        FAT_CHECK_FREE    seq_lens, the columns that each row uses, and rows =
+ *                          ids[0], `count` >= 0 of them
+ *        FAT_CHECK_SHARED  seq_lens, the columns that each row uses, and the groups cu_q [count + 1] with
  *                          the prefixes ids[0] [count]; tokens = queries per
  *                          sequence
  *   host   int64 [FAT_CHECK_HOST_WORDS]: page-locked host memory that the
@@ -750,7 +751,8 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *   10, 11 the first sequence with queries and no keys (-1: none), its queries
  *   12, 13 min and max page id: over every row and the columns below
  *          ceil(max(seq_lens) / page_size) (CACHE, PAGED; INT32_MAX and
- *          INT32_MIN when no column is used), or of the entries
+ *          INT32_MIN when no column is used), of the columns c < ceil(seq_lens[b] /
+ *          page_size) of each row (FREE, SHARED; likewise), or of the entries
  *          [b, clamp(floor(seq_lens[b] / page_size), 0, max_pages - 1)] (APPEND);
  *          the bits of the fp32 min and max, NaN if a value is (RANGE)
  *   7      COPY: 1 a src, 2 a dst out of [0, num_pages), 4 a dst given twice, 8
