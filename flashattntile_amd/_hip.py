@@ -873,21 +873,25 @@ def shared_args(q: torch.Tensor, cache, cu_groups: torch.Tensor, prefix_lens: to
     workspace (:func:`shared_with_args`).  It holds the tensors' addresses."""
     a = SharedArgs()
     k, v, table = cache.k_cache, cache.v_cache, cache.page_table
-    a.q, a.k_cache, a.v_cache, a.k_scale, a.v_scale = _ptr(q), _ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale)
-    a.page_table, a.seq_lens, a.out = _ptr(table), _ptr(cache.seq_lens), _ptr(out)
-    a.cu_groups, a.prefix_lens = _ptr(cu_groups), _ptr(prefix_lens)
+    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.page_table, a.seq_lens = table.data_ptr(), cache.seq_lens.data_ptr()
+    a.cu_groups, a.prefix_lens = cu_groups.data_ptr(), prefix_lens.data_ptr()
     if q.dim() == 4:
-        a.q_stride_t, a.out_stride_t, a.q_len = q.stride(1), out.stride(1), q.shape[1]
-    a.q_stride_b, a.q_stride_h = q.stride(0), q.stride(-2)
-    a.out_stride_b, a.out_stride_h = out.stride(0), out.stride(-2)
-    a.k_stride_page, a.k_stride_slot, a.k_stride_head = k.stride(0), k.stride(1), k.stride(2)
-    a.v_stride_page, a.v_stride_slot, a.v_stride_head = v.stride(0), v.stride(1), v.stride(2)
+        a.batch, a.q_len, a.num_heads, a.head_dim = q.shape
+        a.q_stride_b, a.q_stride_t, a.q_stride_h, _ = q.stride()
+        a.out_stride_b, a.out_stride_t, a.out_stride_h, _ = out.stride()
+    else:
+        a.batch, a.num_heads, a.head_dim = q.shape
+        a.q_stride_b, a.q_stride_h, _ = q.stride()
+        a.out_stride_b, a.out_stride_h, _ = out.stride()
+    a.k_stride_page, a.k_stride_slot, a.k_stride_head, _ = k.stride()
+    a.v_stride_page, a.v_stride_slot, a.v_stride_head, _ = v.stride()
     if k_scale is not None:
-        a.scale_stride_page, a.scale_stride_head = k_scale.stride(0), k_scale.stride(1)
-    a.page_table_stride = table.stride(0)
-    a.batch, a.groups = q.shape[0], prefix_lens.shape[0]
-    a.num_heads, a.num_kv_heads, a.head_dim = q.shape[-2], k.shape[2], q.shape[-1]
-    a.page_size, a.num_pages, a.max_pages = cache.page_size, k.shape[0], table.shape[1]
+        a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        a.scale_stride_page, a.scale_stride_head = k_scale.stride()
+    a.page_table_stride, a.max_pages = table.stride(0), table.shape[1]
+    a.groups = prefix_lens.shape[0]
+    a.num_pages, a.page_size, a.num_kv_heads, _ = k.shape
     a.q_dtype, a.kv_dtype = dtype_code(q.dtype), dtype_code(k.dtype)
     a.softmax_scale = float(softmax_scale)
     return a

@@ -48,7 +48,8 @@ def _check_inputs(q, cache: PagedKVCache, cu_groups, prefix_lens, scales) -> Non
     if cu_groups.shape[0] != prefix_lens.shape[0] + 1 or prefix_lens.shape[0] == 0:
         raise ValueError(f"cu_groups must have one entry more than prefix_lens, at least two; got "
                          f"{cu_groups.shape[0]} and {prefix_lens.shape[0]}")
-    if any(t.device != q.device for t in (cache.k_cache, cache.page_table, cache.seq_lens, cu_groups, prefix_lens)):
+    device = q.device
+    if not (cache.k_cache.device == device == cache.page_table.device == cu_groups.device == prefix_lens.device):
         raise ValueError("q, the cache, its page table, seq_lens, cu_groups and prefix_lens must live on one device")
     quantized = cache.k_cache.dtype in _QUANT_DTYPES
     if quantized != (scales is not None):
@@ -100,18 +101,19 @@ def _assess(r: list[int], q, cache: PagedKVCache) -> None:
 
 def _takes(q, cache: PagedKVCache) -> bool:
     """Whether the shared-prefix kernel takes the launch."""
-    k, v = cache.k_cache, cache.v_cache
-    if q.dtype not in (torch.float16, torch.bfloat16) or cache.head_dim not in (64, 128):
+    if q.dtype not in (torch.float16, torch.bfloat16) or q.shape[-1] not in (64, 128):
         return False
-    if cache.capacity > 2 ** 31 - 4097:
+    k, v, size = cache.k_cache, cache.v_cache, cache.page_size
+    if size >= 2 ** 24 or cache.page_table.shape[1] * size > 2 ** 31 - 4097:
         return False
     eb = k.element_size()
-    if cache.page_size >= 2 ** 24 or any(eb * t.stride(0) >= 2 ** 32 or eb * t.stride(1) >= 2 ** 24 or
-                                         eb * t.stride(1) * cache.page_size >= 2 ** 32 for t in (k, v)):
-        return False
-    words = [k.data_ptr(), v.data_ptr(), q.data_ptr()]
-    words += [eb * s for t in (k, v) for s in t.stride()[:3]]
-    return all(x % 16 == 0 for x in words)
+    bits = k.data_ptr() | v.data_ptr() | q.data_ptr()
+    for t in (k, v):
+        page, slot, head, _ = t.stride()
+        if eb * page >= 2 ** 32 or eb * slot >= 2 ** 24 or eb * slot * size >= 2 ** 32:
+            return False
+        bits |= eb * (page | slot | head)
+    return bits % 16 == 0
 
 
 def _up(n: int, to: int) -> int:
@@ -149,12 +151,19 @@ def _block(q, cache, cu_groups, prefix_lens, scale, scales, out=None):
         raise ValueError("k_cache and v_cache need a contiguous head_dim axis")
     if out is None:
         out = torch.empty_like(q)
-    pt = cache.page_table if cache.page_table.stride(-1) == 1 else cache.page_table.contiguous()
-    sl, cu, pre = cache.seq_lens.contiguous(), cu_groups.contiguous(), prefix_lens.contiguous()
-    dense = PagedKVCache(cache.k_cache, cache.v_cache, pt, sl, cache.page_size)
     sc = None if scales is None else _dense_scales(scales)
-    a = _hip.shared_args(q, dense, cu, pre, out, scale, *((sc["k"], sc["v"]) if sc else ()))
-    return a, out, (q, dense, cu, pre, sc)
+    a = _hip.shared_args(q, cache, cu_groups, prefix_lens, out, scale, *((sc["k"], sc["v"]) if sc else ()))
+    return a, out, sc
+
+
+def _dense(cache: PagedKVCache, cu_groups, prefix_lens):
+    """The cache, groups and prefixes with the table, lengths and lists that the
+    kernels read (unit strides)."""
+    pt, sl = cache.page_table, cache.seq_lens
+    if pt.stride(1) != 1 or not sl.is_contiguous():
+        cache = PagedKVCache(cache.k_cache, cache.v_cache, pt if pt.stride(1) == 1 else pt.contiguous(),
+                             sl.contiguous(), cache.page_size)
+    return cache, cu_groups.contiguous(), prefix_lens.contiguous()
 
 
 def _launch(a, q, cfg: dict, max_group: int, workspace=None) -> None:
@@ -187,6 +196,7 @@ def paged_decode_shared_launch(q: torch.Tensor, cache: PagedKVCache, cu_groups: 
     Takes fp16/bf16 queries at head_dim 64 or 128, else raises.
     """
     with _hip.on_device(q.device):
+        cache, cu_groups, prefix_lens = _dense(cache, cu_groups, prefix_lens)
         a, out, _keep = _block(q, cache, cu_groups, prefix_lens, softmax_scale, scales, out)
         cfg = _resolve(config, q, cache, max_prefix, max_own, max_group or q.shape[0], prefix_lens.shape[0],
                        q.shape[0])
@@ -264,10 +274,9 @@ def paged_decode_attention_shared(
     device = q.device
     with _hip.on_device(device):
         stream = _hip.current_stream_handle(device)
-        sl, pt = cache.seq_lens.contiguous(), cache.page_table
-        pt = pt if pt.stride(-1) == 1 else pt.contiguous()
-        check = _hip.check_begin(_hip.CHECK_SHARED, stream, device, cu_q=cu_groups.contiguous(), seq_lens=sl,
-                                 page_table=pt, page_size=cache.page_size, ids=(prefix_lens.contiguous(),),
+        cache, cu_groups, prefix_lens = _dense(cache, cu_groups, prefix_lens)
+        check = _hip.check_begin(_hip.CHECK_SHARED, stream, device, cu_q=cu_groups, seq_lens=cache.seq_lens,
+                                 page_table=cache.page_table, page_size=cache.page_size, ids=(prefix_lens,),
                                  tokens=tokens)
         # prepared while the check kernel runs
         block = _block(q, cache, cu_groups, prefix_lens, scale, scales) if _takes(q, cache) else None

@@ -174,6 +174,29 @@ def test_rows_of_a_group_and_splits(dtype, kv, sequences):
         assert torch.equal(out, _run(case, config=config))
 
 
+@pytest.mark.parametrize("row_blocks", [1, 4])
+@pytest.mark.parametrize("dtype,kv", [("fp16", "same"), ("bf16", "same"), ("fp16", "fp8"), ("bf16", "fp8"),
+                                      ("fp16", "int8"), ("bf16", "int8")])
+@pytest.mark.parametrize("d", [64, 128])
+def test_every_number_of_rows_of_a_workgroup(row_blocks, dtype, kv, d):
+    """Each kernel at few rows and many, masks of several tokens, scores that rise and fall."""
+    for name, P, tokens in (("ragged", 16, 0), ("edges", 1, 4), ("edges", 64, 2)):
+        if kv != "same" and any(n % P and len(owns) > 1 for n, owns in GROUPS[name]):
+            continue
+        case = _setup(GROUPS[name], P, 2, d, DTYPES[dtype], tokens, 16, kv, seed=row_blocks)
+        label = f"{name} {dtype} {kv} d{d} P{P} T{tokens} row blocks {row_blocks}"
+        print(label, flush=True)
+        out = _run(case, config={"row_blocks": row_blocks})
+        _check(out, *_reference(case["q"], case["cache"], case["scales"]), label)
+    case = _setup([(512, [50, 1, 200] * 12)], 16, 1, d, DTYPES[dtype], 0, 8, seed=6, poison=False)
+    cache = case["cache"]
+    ids = cache.page_table[0, :32].long()
+    ramp = torch.cat([torch.linspace(-3, 3, 256), torch.linspace(3, -3, 256)]).to(DEV).view(32, 16, 1, 1)
+    cache.k_cache[ids] = (case["q"][0, 0].float() * ramp).to(DTYPES[dtype])
+    out = _run(case, softmax_scale=0.3, config={"row_blocks": row_blocks})
+    _check(out, *_reference(case["q"], cache, softmax_scale=0.3), f"scores that rise and fall {row_blocks}")
+
+
 @pytest.mark.parametrize("dtype,kv,P", [("bf16", "same", 16), ("fp16", "int8", 16), ("fp16", "same", 1)])
 def test_long_prefixes(dtype, kv, P):
     print(f"long {dtype} {kv} P{P}", flush=True)
