@@ -35,6 +35,13 @@
  *   fat_cache_stats        the device reductions of validate_cache,
  *                          flashattn_tile/paging.py:84-130 (as called by
  *                          flashattn_tile/kernels/decode.py:503-522)
+ *   fat_paged_decode_shared, fat_copy_pages, fat_fork_sequences,
+ *   fat_free_sequences, fat_compact_pages
+ *                          no reference counterpart: its cache maps every
+ *                          sequence to pages of its own
+ *                          (flashattn_tile/paging.py:133-169), and its decode
+ *                          reads every sequence's own table
+ *                          (flashattn_tile/kernels/decode.py:47-127)
  */
 #ifndef FAT_ABI_H
 #define FAT_ABI_H
