@@ -133,14 +133,14 @@ struct SharedTile {
   static constexpr int NLD = NCH > NT ? NCH / NT : 1;  // per lane
   static constexpr int OS = D + 4;               // row stride (floats) of the key groups' join
   static constexpr int kTile = 32 * (K_RS + V_RS);  // elements
-  // 8-bit caches: the codes are staged as they are (exact in fp16 and bf16) and
-  // k_scale multiplies the fp32 scores.  v_scale multiplies P for bf16, whose
-  // exponents hold any scale; in fp16 the P of a page with a small scale would
-  // lose its bits beside one with a large scale, so V is staged as
-  // round_to_fp16(x * scale) there.
+  // 8-bit caches: the codes are staged as they are, exact in fp16 and bf16.
+  // k_scale multiplies the fp32 scores and v_scale P, whose product with the codes
+  // of V then runs in bf16 for fp16 queries too: its exponents hold any scale,
+  // where in fp16 the P of a page with a small scale would lose its bits beside one
+  // with a large scale, and V times its scale would be rounded once more.
   static constexpr bool FOLD = KV != KV_SAME;
-  static constexpr bool FOLD_V = FOLD && std::is_same<QT, BF16>::value;
-  static constexpr int kScaleFloats = FOLD_V ? 64 : FOLD ? 32 : 0;  // of a tile's keys: K's, V's
+  using VT = typename std::conditional<FOLD, BF16, QT>::type;  // of the second product
+  static constexpr int kScaleFloats = FOLD ? 64 : 0;  // of a tile's keys: K's, V's
   static constexpr int kTileBytes = KG * kBufs * (kTile * 2 + kScaleFloats * 4);
   static constexpr int kJoinBytes = KG > 1 ? (kSharedWaves * 32 * OS + kSharedWaves * 32 * 2) * 4 : 0;
   static constexpr int kBytes = kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes;
@@ -155,10 +155,11 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   using Tl = SharedTile<QT, KV, D, RB>;
   constexpr int KG = Tl::KG, KS = Tl::KS, DB = Tl::DB, K_RS = Tl::K_RS, V_RS = Tl::V_RS, EPC = Tl::EPC, CPR = Tl::CPR,
                 NT = Tl::NT, NCH = Tl::NCH, NLD = Tl::NLD, OS = Tl::OS;
-  constexpr bool FOLD = Tl::FOLD, FOLD_V = Tl::FOLD_V;
+  constexpr bool FOLD = Tl::FOLD;
+  using VT = typename Tl::VT;
   // P enters the second product as bf16 hi + lo parts: one bf16 alone (2^-9) would
   // show beside the output's own rounding where a row sees few keys.
-  constexpr bool SPLIT_P = std::is_same<QT, BF16>::value;
+  constexpr bool SPLIT_P = std::is_same<VT, BF16>::value;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rb = w % RB, kg = w / RB;
@@ -277,37 +278,16 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
       if constexpr (FOLD) R.vsc[i] = vsh[(uint64_t)page[i] * p.sc_sp];
     }
   };
-  // A chunk as QT elements: a copy, the exact values of 8-bit codes, or
-  // (scaled) round_to_QT(float(x) * sc).
-  auto put = [&](uint16_t* dst, const u32x4& raw) __attribute__((always_inline)) {
+  // A chunk as ET elements: a copy, or the exact values of 8-bit codes.
+  auto put = [&](auto et, uint16_t* dst, const u32x4& raw) __attribute__((always_inline)) {
     if constexpr (KV == KV_SAME) {
       *reinterpret_cast<u32x4*>(dst) = raw;
     } else {
       u32 o[8];
-      codes_exact<QT, KV>(raw, o);
+      codes_exact<decltype(et), KV>(raw, o);
       *reinterpret_cast<u32x4*>(dst) = u32x4{o[0], o[1], o[2], o[3]};
       *reinterpret_cast<u32x4*>(dst + 8) = u32x4{o[4], o[5], o[6], o[7]};
     }
-  };
-  auto put_scaled = [&](uint16_t* dst, const u32x4& raw, float sc) __attribute__((always_inline)) {
-    u32 o[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float f[4];
-      if constexpr (KV == KV_I8) {
-        i8x4_biased(raw[j], f);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = __builtin_fmaf(f[e], sc, -128.0f * sc);
-      } else {
-        fp8x4(raw[j], f);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] *= sc;
-      }
-      o[2 * j] = Pair<QT>::pack(f[0], f[1]);
-      o[2 * j + 1] = Pair<QT>::pack(f[2], f[3]);
-    }
-    *reinterpret_cast<u32x4*>(dst) = u32x4{o[0], o[1], o[2], o[3]};
-    *reinterpret_cast<u32x4*>(dst + 8) = u32x4{o[4], o[5], o[6], o[7]};
   };
   uint16_t* const tile0 = reinterpret_cast<uint16_t*>(smem) + kg * Tl::kBufs * Tl::kTile;
   float* const sc0 = reinterpret_cast<float*>(smem + KG * Tl::kBufs * Tl::kTile * 2) + kg * Tl::kBufs * Tl::kScaleFloats;
@@ -317,7 +297,7 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
       const int row = srow + i * (NT / CPR);
-      put(&Kt[row * K_RS + scol * EPC], R.k[i]);
+      put(QT{}, &Kt[row * K_RS + scol * EPC], R.k[i]);
       if constexpr (FOLD) {
         if (scol == 0) sc0[buf * Tl::kScaleFloats + row] = R.ksc[i] * p.scale_log2;
       }
@@ -334,12 +314,8 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
       if constexpr (FOLD) {
         // behind the end: a scale of 0, which the codes' finite values keep at 0
         const float sc = !last || t_begin + 32 * t + row < t_end ? R.vsc[i] : 0.f;
-        if constexpr (FOLD_V) {
-          put(&Vt[row * V_RS + scol * EPC], vv);
-          if (scol == 0) sc0[buf * Tl::kScaleFloats + 32 + row] = sc;
-        } else {
-          put_scaled(&Vt[row * V_RS + scol * EPC], vv, sc);
-        }
+        put(VT{}, &Vt[row * V_RS + scol * EPC], vv);
+        if (scol == 0) sc0[buf * Tl::kScaleFloats + 32 + row] = sc;
       } else {
         if (last) {
           asm volatile("");  // a branch
@@ -348,7 +324,7 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
           const bool in = t_begin + 32 * t + row < t_end;
           vv = u32x4{in ? vv[0] : 0u, in ? vv[1] : 0u, in ? vv[2] : 0u, in ? vv[3] : 0u};
         }
-        put(&Vt[row * V_RS + scol * EPC], vv);
+        put(VT{}, &Vt[row * V_RS + scol * EPC], vv);
       }
     }
   };
@@ -422,7 +398,7 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   f32x4 cv[4];
   auto load_cv = [&](int buf) __attribute__((always_inline)) {
     m_use = m_run == -INFINITY ? 0.f : m_run;
-    if constexpr (FOLD_V) {
+    if constexpr (FOLD) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) cv[j] = *reinterpret_cast<const f32x4*>(&sc0[buf * Tl::kScaleFloats + 32 + 4 * g + 8 * j]);
     }
@@ -431,13 +407,13 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
     float x0 = fast_exp2(FOLD ? s[2 * j] - m_use : __builtin_fmaf(s[2 * j], c, -m_use));
     float x1 = fast_exp2(FOLD ? s[2 * j + 1] - m_use : __builtin_fmaf(s[2 * j + 1], c, -m_use));
     l_run += x0 + x1;
-    if constexpr (FOLD_V) {
+    if constexpr (FOLD) {
       x0 *= cv[j >> 1][2 * (j & 1)];
       x1 *= cv[j >> 1][2 * (j & 1) + 1];
     }
-    const u32 hp = Pair<QT>::pack(x0, x1);
+    const u32 hp = Pair<VT>::pack(x0, x1);
     pf[j >> 2][j & 3] = hp;
-    if constexpr (SPLIT_P) pl[j >> 2][j & 3] = Pair<QT>::pack(x0 - Pair<QT>::lo(hp), x1 - Pair<QT>::hi(hp));
+    if constexpr (SPLIT_P) pl[j >> 2][j & 3] = Pair<VT>::pack(x0 - Pair<VT>::lo(hp), x1 - Pair<VT>::hi(hp));
   };
   // O^T += V^T P^T: entry e is keys 16 u .. + 15 of the tile (u = e / DB), dims 32 db ..
   // + 31 (db = e % DB).
@@ -448,8 +424,8 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
   auto pv = [&](const u32x4& a, int e) __attribute__((always_inline)) {
-    acc[e % DB] = Mfma<QT>::mma(a, pf[e / DB], acc[e % DB]);
-    if constexpr (SPLIT_P) acc[e % DB] = Mfma<QT>::mma(a, pl[e / DB], acc[e % DB]);
+    acc[e % DB] = Mfma<VT>::mma(a, pf[e / DB], acc[e % DB]);
+    if constexpr (SPLIT_P) acc[e % DB] = Mfma<VT>::mma(a, pl[e / DB], acc[e % DB]);
   };
 
   if constexpr (RB == 1) {

@@ -531,8 +531,8 @@ int fat_append_kv(const fat_append_args* args, void* stream);
  * fp16/bf16 queries, head_dim 64 or 128, any page size (FAT_E_UNSUPPORTED
  * otherwise), 16-byte aligned q, K, V and workspace rows.  Lengths, offsets and
  * page ids are clamped on the device: bad ones give wrong answers, never an
- * access out of bounds.  8-bit caches: exact codes, k_scale on the fp32 scores;
- * v_scale on P with bf16 queries, V as round_to_fp16(x * v_scale) with fp16 ones.
+ * access out of bounds.  8-bit caches: exact codes, k_scale on the fp32 scores
+ * and v_scale on P, which then enters the second product as two bf16.
  * The shared keys are cut into prefix_split partials of prefix_chunk keys, a
  * sequence's own into split partials of chunk keys (multiples of 32; the last
  * takes any keys beyond), joined by log-sum-exp through `workspace`, which holds

@@ -1,13 +1,13 @@
 """paged_decode_attention_shared against attention in 64 bits over each sequence's
 own table (which holds the shared pages too).
 
-Tolerance, per element, from the kernel's roundings (``_bound``): P enters the
+Tolerance, per element, from the kernel's roundings (``_reference``): P enters the
 second product as fp16 (half a step, 2^-11 of each p; a p in fp16's subnormals is
-off by 2^-25 of the largest at most, n keys of them) or as two bf16 (2^-16), so
-that a weighted mean of v moves by that share of max |v|; fp32 scores of up to 64
-(log2 units, 2^-24 each, and the sums) move p by less than 2^-16; and the output's
-own rounding is half a step.  8-bit caches are compared on code times scale, with
-fp16 queries on V rounded to fp16 after that.
+off by 2^-25 of the largest at most, n keys of them) or, with bf16 queries and 8-bit
+caches, as two bf16 (2^-16), so that a weighted mean of v moves by that share of max
+|v|; fp32 scores of up to 64 (log2 units, 2^-24 each, and the sums) move p by less
+than 2^-16; and the output's own rounding is half a step.  8-bit caches are compared
+on code times scale.
 """
 
 from __future__ import annotations
@@ -81,23 +81,15 @@ def _setup(groups, P, hkv, d, dtype, tokens=1, heads=8, kv="same", seed=0, spare
             "scales": None if scales is None else {n: t.to(DEV) for n, t in scales.items()}}
 
 
-def _values(cache, scales, dtype):
+def _values(cache, scales):
     """K and V pages in 64 bits."""
-    out = []
-    for name, x in (("k", cache.k_cache), ("v", cache.v_cache)):
-        if scales is None:
-            out.append(x.double().cpu())
-            continue
-        y = x.double().cpu() * scales[name].double().cpu()[:, None, :, None]
-        if name == "v" and dtype == torch.float16:
-            y = (x.float().cpu() * scales[name].cpu()[:, None, :, None]).half().double()
-        out.append(y)
-    return out
+    pages = {"k": cache.k_cache.double().cpu(), "v": cache.v_cache.double().cpu()}
+    return [x if scales is None else x * scales[n].double().cpu()[:, None, :, None] for n, x in pages.items()]
 
 
 def _reference(q, cache, scales=None, softmax_scale=None):
     """Output and its bound, in 64 bits."""
-    k, v = _values(cache, scales, q.dtype)
+    k, v = _values(cache, scales)
     q4 = (q if q.dim() == 4 else q[:, None]).double().cpu()
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
     batch, tokens, heads, d = q4.shape
@@ -105,7 +97,8 @@ def _reference(q, cache, scales=None, softmax_scale=None):
     out, bound = torch.zeros_like(q4), torch.zeros_like(q4)
     table = cache.page_table.cpu().long()
     part = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -16, torch.float32: 2.0 ** -18}[q.dtype]
-    tiny = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    part = part if scales is None else 2.0 ** -16
+    tiny = 2.0 ** -25 if q.dtype == torch.float16 and scales is None else 0.0
     half = torch.finfo(q.dtype).eps / 2
     for b, n in enumerate(cache.seq_lens.tolist()):
         ids = table[b, :math.ceil(n / cache.page_size)]
