@@ -187,10 +187,11 @@ def paged_decode_shared_launch(q: torch.Tensor, cache: PagedKVCache, cu_groups: 
     """Enqueue the shared-prefix decode without validation or synchronisation
     (capture, serving loops that validated once).
 
-    ``max_prefix`` and ``max_own`` bound the groups' prefixes and the keys
-    behind them, ``max_group`` the sequences of a group (default: the batch);
-    they size the grid, and more keys than they say are still attended.
-    Lengths, table, groups and prefixes are read on the device at every run.
+    ``max_prefix`` and ``max_own`` are the groups' longest prefix and the most
+    keys behind one; they size the grid, and more keys than they say are still
+    attended.  No group may have more sequences than ``max_group`` (default: the
+    batch): the outputs of those beyond are undefined.  Lengths, table, groups
+    and prefixes are read on the device at every run.
     ``q`` must be contiguous; ``out`` and ``workspace`` (uint8, 4 x rows x heads
     x partials x (head_dim + 2) bytes) may be passed in to avoid allocations.
     Takes fp16/bf16 queries at head_dim 64 or 128, else raises.
