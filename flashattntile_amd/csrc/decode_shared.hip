@@ -169,6 +169,21 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   const int R = n_seq * per_seq;
   const int n_tiles = t_end > t_begin ? (t_end - t_begin + 31) >> 5 : 0;
 
+  auto row_of = [&](int r) {  // global row of row r of the item
+    const int s = r / per_seq;
+    const int in = r - s * per_seq;
+    const int t = in / p.group;
+    return ((int64_t)(b0 + s) * p.T + t) * p.H + kvh * p.group + (in - t * p.group);
+  };
+  if (n_tiles == 0) {  // uniform: partials of weight 0, whose acc the join leaves alone
+    for (int r = row0 + threadIdx.x; r < min(row0 + 32 * RB, R); r += kSharedWaves * 64) {
+      const int64_t at = row_of(r) * S + slot;
+      p.ws_ml[2 * at] = -INFINITY;
+      p.ws_ml[2 * at + 1] = 0.f;
+    }
+    return;
+  }
+
   // This lane's row, and the end of its visible keys: token t of a sequence of
   // len keys sees those before len - T + 1 + t.
   const int my_row = min(row0 + 32 * rb + li, R - 1);
@@ -539,12 +554,6 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   }
 
   const float l_tot = xor32<OpAdd>(l_run);
-  auto row_of = [&](int r) {  // global row of row r of the item
-    const int s = r / per_seq;
-    const int in = r - s * per_seq;
-    const int t = in / p.group;
-    return ((int64_t)(b0 + s) * p.T + t) * p.H + kvh * p.group + (in - t * p.group);
-  };
   if constexpr (KG == 1) {
     if (row0 + 32 * rb + li < R) {
       const int64_t at = row_of(row0 + 32 * rb + li) * S + slot;
@@ -638,11 +647,15 @@ void decode_shared_kernel(const SharedParams p) {
     return;
   }
   const int id = blockIdx.x - p.prefix_blocks;
-  const int per_b = p.split * p.Hkv * p.own_tiles;
-  const int b = id / per_b;
-  const int r = id - b * per_b;
-  const int slot = r / (p.Hkv * p.own_tiles);
-  const int y = r - slot * (p.Hkv * p.own_tiles);
+  // The slots of a sequence lie far apart: workgroups go to the XCDs and to their
+  // shader engines in turn, and where many sequences have no keys in their second
+  // half, slots side by side would leave every other engine idle (128 sequences of 100
+  // to 2000 bf16 keys in four chunks: 111 us so, 77 apart).
+  const int per_b = p.Hkv * p.own_tiles;
+  const int slot = id / (p.B * per_b);
+  const int r = id - slot * (p.B * per_b);
+  const int b = r / per_b;
+  const int y = r - b * per_b;
   const int kvh = y / p.own_tiles;
   const int tile = y - kvh * p.own_tiles;
   const int grp = group_of(p.cu, p.G, b);

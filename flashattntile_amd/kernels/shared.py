@@ -13,6 +13,8 @@ sequence's own table, ``kernels/decode.py:47-127``).
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .. import _hip
@@ -121,21 +123,29 @@ def _up(n: int, to: int) -> int:
 
 
 def shared_splits(num_kv_heads: int, group_rows: int, own_tiles: int, groups: float, max_prefix: int,
-                  sequences: float, max_own: int) -> dict:
+                  sequences: float, max_own: int, rows: int) -> dict:
     """Partials of a launch: ``prefix_split`` x ``prefix_chunk`` keys of every
     prefix, ``split`` x ``chunk`` own keys of every sequence.
 
     ``group_rows``: query rows of the largest group and KV head; ``own_tiles``:
-    32-row tiles of a sequence.  ``groups`` and ``sequences`` count those of the
-    longest's length (the sum of all lengths by the longest): splits that fit the
-    longest leave the chip to the others' few workgroups otherwise.
+    32-row tiles of a sequence; ``rows``: query rows of all heads.  ``groups`` and
+    ``sequences`` count those of the longest's length (the sum of all lengths by the
+    longest): splits that fit the longest leave the chip to the others' few
+    workgroups otherwise.
     """
-    wide = group_rows > 32
-    # 128 rows: one workgroup per CU (its tiles fill the LDS port), 512 keys each at least.
-    rows, keys, want = (128, 512, 256) if wide else (32, 256, 512)
-    tiles = -(-group_rows // rows)
-    prefix_split = max(1, min(round(want / max(1.0, groups * num_kv_heads * tiles)), 64, max_prefix // keys))
-    split = max(1, min(int(512 / max(1.0, sequences * num_kv_heads * own_tiles)), 64, max_own // 256))
+    # n chunks of K keys cost a chain of a K / n us, and n b for their partials (1040
+    # bytes per row, written and read) and workgroups: least at sqrt(a K / b), a little
+    # below as the chunks overlap.  No more workgroups than CUs.  Chunks taken, us at
+    # 1 chunk, at them and at twice them (fp16, 8 KV heads): 1 group of 8 rows x 4096
+    # keys 17: 52.5, 12.8, 14.2; of 256 x 1024 5: 35.3, 19.0, 21.2; 4 of 128 x 2048 5:
+    # 59.9, 31.0, 37.2; 1 of 512 x 32768 8: 170 (16: 180).
+    tile, per_key = (128, 0.022) if group_rows > 32 else (32, 0.0105)
+    items = max(1.0, groups * num_kv_heads * -(-group_rows // tile))
+    best = 0.8 * math.sqrt(per_key * max_prefix / (2.0e-4 * rows + 0.01 * items))
+    prefix_split = max(1, min(round(min(best, 256 / items)), 64, max_prefix // 32))
+    # Four workgroups of own keys per CU (128 sequences of 100 to 2000 keys on fp8: 1
+    # chunk 66.6 us, 2 60.4, 4 62.7, 8 72.6).
+    split = max(1, min(int(1024 / max(1.0, sequences * num_kv_heads * own_tiles)), 64, max_own // 256))
     return _chunks(prefix_split, split, max_prefix, max_own)
 
 
@@ -209,7 +219,7 @@ def _resolve(config, q, cache, max_prefix: int, max_own: int, max_group: int, gr
              sequences: float) -> dict:
     per_seq = (q.shape[1] if q.dim() == 4 else 1) * q.shape[-2] // cache.num_kv_heads
     cfg = shared_splits(cache.num_kv_heads, max_group * per_seq, -(-per_seq // 32), groups, max_prefix, sequences,
-                        max_own)
+                        max_own, q.shape[0] * per_seq * cache.num_kv_heads)
     given = _given(config) if config else None
     if not given:
         return cfg

@@ -115,18 +115,21 @@ def test_splits_cover_every_length(prefix, own):
         for rows in (1, 32, 33, 4096):
             for groups in (1.0, 3.7, 500.0):
                 for sequences in (1.0, 17.5, 4000.0):
-                    _uses(shared_splits(hkv, rows, -(-rows // 32), groups, prefix, sequences, own), prefix, own)
+                    _uses(shared_splits(hkv, rows, -(-rows // 32), groups, prefix, sequences, own, 32 * rows), prefix,
+                          own)
 
 
 def test_splits_fill_the_chip_and_no_more():
     # one long prefix of 128 sequences x 4 rows: 8 heads x 4 tiles of 128 rows x 8 = 256 workgroups
-    assert shared_splits(8, 512, 1, 1.0, 32768, 128.0, 2000)["prefix_split"] == 8
-    # a chunk has 512 keys at least where 128 rows share them, 256 where 32 do
-    assert shared_splits(8, 128, 1, 1.0, 4096, 32.0, 1000)["prefix_split"] == 8
-    assert shared_splits(8, 16, 1, 1.0, 512, 4.0, 60)["prefix_split"] == 2
-    # many sequences need no split of their own keys
-    assert shared_splits(8, 512, 1, 1.0, 32768, 128.0, 2000)["split"] == 1
-    assert shared_splits(8, 16, 1, 1.0, 512, 2.0, 100000)["split"] == 32
+    assert shared_splits(8, 512, 1, 1.0, 32768, 128.0, 2000, 4096)["prefix_split"] == 8
+    # few rows are worth more partials than many
+    few, many = (shared_splits(8, rows, 1, 1.0, 4096, 8.0, 100, 8 * rows)["prefix_split"] for rows in (8, 128))
+    assert 8 <= many < few <= 24
+    assert shared_splits(8, 8, 1, 1.0, 31, 2.0, 100, 64)["prefix_split"] == 1
+    # many sequences need no split of their own keys, few do, in chunks of 256 at least
+    assert shared_splits(8, 512, 1, 1.0, 32768, 128.0, 2000, 4096)["split"] == 1
+    assert shared_splits(8, 16, 1, 1.0, 512, 2.0, 100000, 64)["split"] == 64
+    assert shared_splits(8, 16, 1, 1.0, 512, 2.0, 1000, 64)["split"] == 3
 
 
 @pytest.mark.gpu
