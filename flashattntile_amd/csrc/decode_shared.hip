@@ -858,6 +858,16 @@ extern "C" int fat_paged_decode_shared(const fat_shared_args* a, void* stream_pt
                         need, (long long)a->workspace_bytes);
     return FAT_E_INVALID;
   }
+  // Partials are written while the launch's other buffers are read.
+  const uintptr_t ws = (uintptr_t)a->workspace;
+  for (const void* p : {a->q, a->k_cache, a->v_cache, (const void*)a->k_scale, (const void*)a->v_scale,
+                        (const void*)a->page_table, (const void*)a->seq_lens, (const void*)a->cu_groups,
+                        (const void*)a->prefix_lens, (const void*)a->out}) {
+    if ((uintptr_t)p >= ws && (uintptr_t)p < ws + need) {
+      fat_host::set_error("fat_paged_decode_shared: the workspace overlaps another buffer of the launch");
+      return FAT_E_INVALID;
+    }
+  }
   fat::SharedParams prm{};
   prm.q = static_cast<const uint8_t*>(a->q);
   prm.k = static_cast<const uint8_t*>(a->k_cache);

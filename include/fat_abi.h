@@ -538,7 +538,8 @@ int fat_append_kv(const fat_append_args* args, void* stream);
  * takes any keys beyond), joined by log-sum-exp through `workspace`, which holds
  * fat_paged_decode_shared_workspace_bytes(batch * q_len, num_heads, head_dim,
  * prefix_split + split) bytes.  Launches that may run at the same time need one
- * each.  max_group: no group has more sequences (outputs beyond are undefined).
+ * each; no other buffer of the launch may begin in it.  max_group: no group has
+ * more sequences (outputs beyond are undefined).
  */
 typedef struct fat_shared_args {
   const void* q;
