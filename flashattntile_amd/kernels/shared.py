@@ -118,6 +118,14 @@ def _takes(q, cache: PagedKVCache) -> bool:
     return bits % 16 == 0
 
 
+def _ordinary_takes(cache: PagedKVCache, tokens: int) -> bool:
+    """Whether ordinary decode takes a 16-bit launch that the shared-prefix kernel
+    takes: with several tokens its MFMA kernel, on power-of-two pages of at least
+    the rows that one of its loads covers."""
+    size = cache.page_size
+    return tokens == 1 or (size & (size - 1) == 0 and size >= (4 if cache.head_dim == 128 else 8))
+
+
 def _up(n: int, to: int) -> int:
     return -(-n // to) * to
 
@@ -295,7 +303,7 @@ def paged_decode_attention_shared(
         _assess(r, q, cache)
         # Nothing is shared: 64 sequences of 4100 keys took 221 us here, 195 as ordinary
         # decode (which rounds an 8-bit cache's scaled values to bf16, and so isn't taken there).
-        if block is None or (r[9] == r[11] and scales is None and not given):
+        if block is None or (r[9] == r[11] and scales is None and not given and _ordinary_takes(cache, tokens)):
             cfg = _resolve_config(None, q, cache, r[1], r[2], q_len=tokens)
             return _decode(q, cache, scale, cfg, None, None if scales is None else _dense_scales(scales))
         a, out, keep = block
