@@ -126,6 +126,16 @@ def _ordinary_takes(cache: PagedKVCache, tokens: int) -> bool:
     return tokens == 1 or (size & (size - 1) == 0 and size >= (4 if cache.head_dim == 128 else 8))
 
 
+def _one_by_one(q, cache: PagedKVCache):
+    """Every token of a multi-token call as a sequence of its own, for the kernels
+    that take one query per sequence: token t sees the first len - T + 1 + t keys."""
+    batch, tokens, heads, dim = q.shape
+    lens = cache.seq_lens[:, None] + torch.arange(1 - tokens, 1, dtype=torch.int32, device=q.device)
+    table = cache.page_table[:, None].expand(-1, tokens, -1).reshape(batch * tokens, -1)
+    return q.view(batch * tokens, heads, dim), PagedKVCache(cache.k_cache, cache.v_cache, table, lens.view(-1),
+                                                            cache.page_size)
+
+
 def _up(n: int, to: int) -> int:
     return -(-n // to) * to
 
@@ -278,9 +288,10 @@ def paged_decode_attention_shared(
     partials per prefix and per sequence (default: by the lengths).
 
     Shapes that the kernel isn't built for (fp32, other head_dims than 64 and
-    128, rows that aren't 16-byte aligned) run as ordinary decode, which reads
-    the prefix once per sequence, and so do batches without ``scales`` in which no
-    two sequences share a key.  Returns ``q``'s shape and dtype.
+    128) run as ordinary decode, which reads the prefix once per sequence, and per
+    token of a multi-token query, and so do batches without ``scales`` in which no
+    two sequences share a key; ``config`` does not apply to the former.  K and V
+    rows are 16-byte aligned, as for every decode.  Returns ``q``'s shape and dtype.
     """
     _check_inputs(q, cache, cu_groups, prefix_lens, scales)
     _require_rocm(q, cache, "paged_decode_attention_shared")
@@ -304,8 +315,12 @@ def paged_decode_attention_shared(
         # Nothing is shared: 64 sequences of 4100 keys took 221 us here, 195 as ordinary
         # decode (which rounds an 8-bit cache's scaled values to bf16, and so isn't taken there).
         if block is None or (r[9] == r[11] and scales is None and not given and _ordinary_takes(cache, tokens)):
-            cfg = _resolve_config(None, q, cache, r[1], r[2], q_len=tokens)
-            return _decode(q, cache, scale, cfg, None, None if scales is None else _dense_scales(scales))
+            pages, shape = r[2], q.shape
+            if block is None and tokens > 1:
+                q, cache = _one_by_one(q, cache)
+                pages, tokens = pages * tokens, 1
+            cfg = _resolve_config(None, q, cache, r[1], pages, q_len=tokens)
+            return _decode(q, cache, scale, cfg, None, None if scales is None else _dense_scales(scales)).view(shape)
         a, out, keep = block
         cfg = _resolve(config, q, cache, r[6], r[8], max(1, r[5]), r[9] / max(1, r[6]), r[10] / max(1, r[8]))
         _launch(a, q, cfg, max(1, r[5]))
