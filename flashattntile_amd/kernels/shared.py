@@ -109,7 +109,7 @@ def _takes(q, cache: PagedKVCache) -> bool:
     if size >= 2 ** 24 or cache.page_table.shape[1] * size > 2 ** 31 - 4097:
         return False
     eb = k.element_size()
-    bits = k.data_ptr() | v.data_ptr() | q.data_ptr()
+    bits = k.data_ptr() | v.data_ptr()
     for t in (k, v):
         page, slot, head, _ = t.stride()
         if eb * page >= 2 ** 32 or eb * slot >= 2 ** 24 or eb * slot * size >= 2 ** 32:
@@ -184,6 +184,15 @@ def _block(q, cache, cu_groups, prefix_lens, scale, scales, out=None):
     return a, out, sc
 
 
+def _dense_query(q: torch.Tensor) -> torch.Tensor:
+    """``q`` with the strides of its shape (torch calls a tensor contiguous whatever
+    those of its axes of one entry are), on a 16-byte boundary."""
+    q = q.contiguous()
+    if q.data_ptr() % 16:
+        return q.clone(memory_format=torch.contiguous_format)
+    return q.view(-1).view(q.shape) if 1 in q.shape else q
+
+
 def _dense(cache: PagedKVCache, cu_groups, prefix_lens):
     """The cache, groups and prefixes with the table, lengths and lists that the
     kernels read (unit strides)."""
@@ -220,11 +229,13 @@ def paged_decode_shared_launch(q: torch.Tensor, cache: PagedKVCache, cu_groups: 
     attended.  No group may have more sequences than ``max_group`` (default: the
     batch): the outputs of those beyond are undefined.  Lengths, table, groups
     and prefixes are read on the device at every run.
-    ``q`` must be contiguous; ``out`` and ``workspace`` (uint8, 4 x rows x heads
-    x partials x (head_dim + 2) bytes) may be passed in to avoid allocations.
+    ``q`` must be contiguous and begin on a 16-byte boundary (else it is copied);
+    ``out`` and ``workspace`` (uint8, 4 x rows x heads x partials x (head_dim + 2)
+    bytes) may be passed in to avoid allocations.
     Takes fp16/bf16 queries at head_dim 64 or 128, else raises.
     """
     with _hip.on_device(q.device):
+        q = _dense_query(q)
         cache, cu_groups, prefix_lens = _dense(cache, cu_groups, prefix_lens)
         a, out, _keep = _block(q, cache, cu_groups, prefix_lens, softmax_scale, scales, out)
         cfg = _resolve(config, q, cache, max_prefix, max_own, max_group or q.shape[0], prefix_lens.shape[0],
@@ -300,9 +311,9 @@ def paged_decode_attention_shared(
     tokens = q.shape[1] if q.dim() == 4 else 1
     given = _given(config)
     scale = _scale_of(q, softmax_scale)
-    q = q.contiguous()
     device = q.device
     with _hip.on_device(device):
+        q = _dense_query(q)
         stream = _hip.current_stream_handle(device)
         cache, cu_groups, prefix_lens = _dense(cache, cu_groups, prefix_lens)
         check = _hip.check_begin(_hip.CHECK_SHARED, stream, device, cu_q=cu_groups, seq_lens=cache.seq_lens,

@@ -1,6 +1,6 @@
 """paged_decode_attention_shared where ordinary decode could run in its place:
-batches in which nothing is shared, and several tokens per sequence on types and
-head_dims that ordinary multi-token decode doesn't take.
+batches in which nothing is shared, several tokens per sequence on pages and types
+that ordinary multi-token decode doesn't take, and queries of any alignment.
 
 Tolerance: test_gpu_decode_shared's, whose terms cover ordinary decode too (its
 kernels for one query keep P in fp32)."""
@@ -13,7 +13,8 @@ import torch
 from test_gpu_decode_shared import DTYPES, _check, _ints, _reference, _run, _setup
 
 import flashattntile_amd as fat
-from flashattntile_amd import PagedKVCache
+from flashattntile_amd import PagedKVCache, paged_decode_attention_shared
+from flashattntile_amd.kernels.shared import paged_decode_shared_launch
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +72,32 @@ def test_several_tokens_of_shapes_that_run_as_ordinary_decode(dtype, d, kv, head
         assert torch.equal(out.view(q.shape), fat.paged_decode_attention(q, cache))
     else:
         assert torch.equal(out.view(q.shape), fat.paged_decode_attention_fp8(q, cache, case["scales"]))
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 3])
+@pytest.mark.parametrize("groups", [[(32, [20])], [(48, [5, 9])], [(0, [7, 40])]])
+def test_queries_behind_any_address(tokens, groups):
+    """Queries that begin between 16-byte boundaries, and those whose axes of one
+    entry have odd strides (torch calls both contiguous)."""
+    print(f"addresses {tokens} {groups}", flush=True)
+    for heads, hkv in ((8, 2), (1, 1)):
+        case = _setup(groups, 16, hkv, 64, torch.float16, tokens, heads, seed=tokens)
+        q = case["q"]
+        want = _run(case)
+        _check(want, *_reference(q, case["cache"]), "as it was")
+        room = torch.zeros(q.numel() + 40, dtype=q.dtype, device="cuda")
+        views = []
+        for offset in (1, 3, 8):
+            flat = room.clone()
+            flat[offset:offset + q.numel()] = q.flatten()
+            views.append(flat[offset:offset + q.numel()].view(q.shape))
+        odd = q.clone()
+        views.append(odd.as_strided(q.shape, [s if n > 1 else s + 13 for n, s in zip(q.shape, q.stride())]))
+        for i, view in enumerate(views):
+            assert view.is_contiguous()
+            out = paged_decode_attention_shared(view, case["cache"], case["cu_groups"], case["prefix_lens"])
+            assert torch.equal(out, want), i
+        config = {"prefix_split": 2, "split": 2}
+        a, b = (paged_decode_shared_launch(x, case["cache"], case["cu_groups"], case["prefix_lens"], 0.125, 48, 40,
+                                           config=config) for x in (q, views[-1]))
+        assert torch.equal(a, b)
