@@ -264,9 +264,10 @@ __global__ __launch_bounds__(kCheckThreads) void check_kernel(const CheckParams 
 // FREE and SHARED: workgroup 0 reduces the lengths (and the rows to free, the
 // groups, their prefixes), the others' waves take the used columns of the table,
 // SHARED with a comparison of those that a prefix fills with the group's first row
-// (a difference makes the smallest id INT_MIN).  A row's columns go to `per_row`
-// waves in turn, so no entry costs a division and few long rows spread as well as
-// many short ones: 512 rows of up to 8000 ids take 8 us, 4 rows 5.
+// (a difference makes the smallest id INT_MIN, which stands for nothing else).  A
+// row's columns go to `per_row` waves in turn, so no entry costs a division and few
+// long rows spread as well as many short ones: 512 rows of up to 8000 ids take 8 us,
+// 4 rows 5.
 constexpr int kRowsThreads = 1024;
 constexpr int kRowsWaves = kRowsThreads / 64;
 constexpr int64_t kRowsEntries = 4096;  // table entries per workgroup
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(kRowsThreads) void check_rows_kernel(const CheckPar
         }
       }
     }
-    range[0] = differs ? INT_MIN : pmn;
+    range[0] = differs ? INT_MIN : SHARED ? max(pmn, INT_MIN + 1) : pmn;
     range[1] = pmx;
     const long long r = rows_reduce(range, range_op, kRowsWaves);
     range[0] = r;

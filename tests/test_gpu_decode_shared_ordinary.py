@@ -101,3 +101,13 @@ def test_queries_behind_any_address(tokens, groups):
         a, b = (paged_decode_shared_launch(x, case["cache"], case["cu_groups"], case["prefix_lens"], 0.125, 48, 40,
                                            config=config) for x in (q, views[-1]))
         assert torch.equal(a, b)
+
+
+def test_a_page_id_that_is_the_smallest_number():
+    """-2^31 in a used column is a negative page, not a page that isn't shared."""
+    case = _setup([(48, [5, 9]), (32, [20])], 16, 2, 64, torch.float16, 0, 8, seed=10)
+    table = case["cache"].page_table.clone()
+    table[2, 1] = -2 ** 31
+    cache = PagedKVCache(case["cache"].k_cache, case["cache"].v_cache, table, case["cache"].seq_lens, 16)
+    with pytest.raises(AssertionError, match="negative page id"):
+        paged_decode_attention_shared(case["q"], cache, case["cu_groups"], case["prefix_lens"])
