@@ -12,6 +12,9 @@
 //   own items     the rows of one sequence x a chunk of the keys behind N, read
 //                 through its own table row;
 // and a second kernel joins them, a row's partials in the order of its keys.
+// On 8-bit caches N is the prefix's whole pages: the page that it ends in has one
+// scale for the shared keys and those behind them, so every sequence has other
+// codes of them there.
 //
 // What bounds it: own items stream K and V once (HBM: 128 sequences x 630 bf16
 // keys, 8 KV heads, D 128 take 63 us, 5.2 TB/s); a prefix item does 4 x 32 RB x D
@@ -615,6 +618,12 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   }
 }
 
+// The keys of a prefix of n that are read once for its group.
+template <int KV>
+__device__ __forceinline__ int shared_keys(const SharedParams& p, int n) {
+  return KV == KV_SAME ? n : n - n % p.P;
+}
+
 template <typename QT, int KV, int D, int RB>
 __global__ __launch_bounds__(kSharedWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void decode_shared_kernel(const SharedParams p) {
@@ -640,7 +649,7 @@ void decode_shared_kernel(const SharedParams p) {
     const int b1 = min(max(p.cu[grp + 1], b0), p.B);
     const int row0 = tile * 32 * RB;
     if (row0 >= (b1 - b0) * p.T * p.group) return;
-    const int n = min(max(p.prefix[grp], 0), cap);
+    const int n = shared_keys<KV>(p, min(max(p.prefix[grp], 0), cap));
     const int t_begin = min(slot * p.prefix_chunk, n);
     const int t_end = slot == p.prefix_split - 1 ? n : min(t_begin + p.prefix_chunk, n);
     shared_segment<QT, KV, D, RB>(p, smem, b0, b1 - b0, kvh, row0, p.pt + (int64_t)b0 * p.pt_sb, t_begin, t_end, slot, S);
@@ -660,7 +669,7 @@ void decode_shared_kernel(const SharedParams p) {
   const int tile = y - kvh * p.own_tiles;
   const int grp = group_of(p.cu, p.G, b);
   const int len = min(max(p.lens[b], 0), cap);
-  const int n = grp < 0 ? 0 : min(max(p.prefix[grp], 0), len);
+  const int n = grp < 0 ? 0 : min(shared_keys<KV>(p, min(max(p.prefix[grp], 0), cap)), len);
   const int t_begin = min((int64_t)n + (int64_t)slot * p.chunk, (int64_t)len);
   const int t_end = slot == p.split - 1 ? len : min((int64_t)t_begin + p.chunk, (int64_t)len);
   shared_segment<QT, KV, D, 1>(p, smem, b, 1, kvh, tile * 32, p.pt + (int64_t)b * p.pt_sb, t_begin, t_end,

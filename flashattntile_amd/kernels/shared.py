@@ -295,7 +295,8 @@ def paged_decode_attention_shared(
     sequence then has its own copy of that page, as
     :func:`~flashattntile_amd.page_ops.fork_sequences` makes it), the pages it
     fills must be the same ids in all rows of the group.  ``scales`` selects an
-    int8 / float8_e4m3fn cache.  ``config``: ``prefix_split`` and ``split``,
+    int8 / float8_e4m3fn cache, where that last page is read per sequence (its scale
+    and codes depend on each one's own keys).  ``config``: ``prefix_split`` and ``split``,
     partials per prefix and per sequence (default: by the lengths).
 
     Shapes that the kernel isn't built for (fp32, other head_dims than 64 and
@@ -333,7 +334,12 @@ def paged_decode_attention_shared(
             cfg = _resolve_config(None, q, cache, r[1], pages, q_len=tokens)
             return _decode(q, cache, scale, cfg, None, None if scales is None else _dense_scales(scales)).view(shape)
         a, out, keep = block
-        cfg = _resolve(config, q, cache, r[6], r[8], max(1, r[5]), r[9] / max(1, r[6]), r[10] / max(1, r[8]))
+        prefix, own = r[6], r[8]
+        groups, sequences = r[9] / max(1, prefix), r[10] / max(1, own)
+        if scales is not None:  # a prefix's last page is among its sequences' own keys
+            own = min(r[1], own + min(prefix, cache.page_size - 1))
+            prefix -= prefix % cache.page_size
+        cfg = _resolve(config, q, cache, prefix, own, max(1, r[5]), groups, sequences)
         _launch(a, q, cfg, max(1, r[5]))
         del keep
         return out

@@ -525,9 +525,11 @@ int fat_append_kv(const fat_append_args* args, void* stream);
  * Sequences cu_groups[g] .. cu_groups[g + 1] - 1 are group g (cu_groups[0] = 0,
  * non-decreasing, cu_groups[groups] = batch); their first prefix_lens[g] keys
  * are the same, and are read through the table row of the group's first
- * sequence.  seq_lens counts all keys, the shared ones among them; prefix_lens[g]
- * <= seq_lens[b] - q_len + 1.  A prefix of 0 keys and groups of one or no
- * sequence are valid.  Layouts and q_len as for fat_paged_decode;
+ * sequence (8-bit caches: those in pages that the prefix fills; the page that it
+ * ends in has another scale, and so other codes, in every sequence, and is read
+ * through each one's own row).  seq_lens counts all keys, the shared ones among
+ * them; prefix_lens[g] <= seq_lens[b] - q_len + 1.  A prefix of 0 keys and groups
+ * of one or no sequence are valid.  Layouts and q_len as for fat_paged_decode;
  * fp16/bf16 queries, head_dim 64 or 128, any page size (FAT_E_UNSUPPORTED
  * otherwise), 16-byte aligned q, K, V and workspace rows.  Lengths, offsets and
  * page ids are clamped on the device: bad ones give wrong answers, never an
