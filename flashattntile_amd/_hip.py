@@ -22,7 +22,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libfat_hip.so"
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 # enum fat_dtype
 DT_F16 = 0

@@ -436,7 +436,9 @@ __global__ __launch_bounds__(kRowsThreads) void check_rows_kernel(const CheckPar
 // workgroup marks a list's ids in a bitmap in LDS, 2^19 ids at a time (a pool of
 // more takes several turns over the list): the bit that was there before is a
 // repetition, and the other list's ids are looked up in it.  8192 pairs take 7.6
-// us (30 with the owners of the ids in device memory), 16 pairs 2.5.
+// us (30 with the owners of the ids in device memory), 16 pairs 2.5.  FORK: the
+// other workgroups mark the pages that the forks take, and look the used columns
+// of all rows up among them (one that is makes the smallest id INT_MIN).
 constexpr int kListThreads = 1024;
 constexpr int kListIds = 1 << 19;
 
@@ -465,6 +467,49 @@ __global__ __launch_bounds__(kListThreads) void check_lists_kernel(const CheckPa
     len = (unsigned)parent < (unsigned)limit ? p.lens[parent] : 0;
     return len > 0 && len <= (int64_t)p.max_pages * p.P && len % p.P != 0;
   };
+  auto finish = [&](int word, long long v) {
+    auto put = [&](int at, long long x) {
+      __hip_atomic_store(p.host + at, (int64_t)x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    };
+    put(word, v);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the result is complete
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    put(FAT_CHECK_RESULTS + 2 * blockIdx.x + 1, p.ticket);
+  };
+  if constexpr (FORK) {
+    if (blockIdx.x > 0) {  // uniform
+      const int lane = tid & 63;
+      const int workers = ((int)gridDim.x - 1) * (kListThreads / 64);
+      const int worker = ((int)blockIdx.x - 1) * (kListThreads / 64) + __builtin_amdgcn_readfirstlane(tid >> 6);
+      const int per_row = max(1, workers / p.B);
+      bool found = false;
+      for (int base = 0; base < p.num_pages; base += min(kListIds, p.num_pages - base)) {
+        const unsigned ids = min(kListIds, p.num_pages - base);
+        clear(ids);
+        for (int i = tid; i < n; i += kListThreads) {
+          int len;
+          if (tail(i, len) && pages[i] >= base && (unsigned)(pages[i] - base) < ids) mark(pages[i] - base);
+        }
+        __syncthreads();
+        for (long long u = worker; u < (long long)p.B * per_row; u += workers) {
+          const int r = (int)(u / per_row);
+          const int32_t* row = p.pt + r * p.pt_sb;
+          const int64_t used = ((int64_t)max(p.lens[r], 0) + p.P - 1) / p.P;
+          const int cols = (int)min(used, (int64_t)p.max_pages);
+#pragma unroll 8
+          for (long long c = (u - (long long)r * per_row) * 64 + lane; c < cols; c += per_row * 64) {
+            const int id = row[c];
+            if (id >= base && (unsigned)(id - base) < ids) found |= (bits[(id - base) >> 5] >> ((id - base) & 31)) & 1;
+          }
+        }
+      }
+      if (found) s_flags = 1;
+      __syncthreads();
+      if (tid == 0) finish(FAT_CHECK_RESULTS + 2 * blockIdx.x, s_flags ? (long long)(uint32_t)INT_MIN : (long long)INT_MAX);
+      return;
+    }
+  }
   for (int base = 0; base < limit; base += min(kListIds, limit - base)) {
     const unsigned ids = min(kListIds, limit - base);
     clear(ids);
@@ -506,14 +551,8 @@ __global__ __launch_bounds__(kListThreads) void check_lists_kernel(const CheckPa
   if (flags) atomicOr(&s_flags, flags);
   __syncthreads();
   if (tid == 0) {
-    auto put = [&](int word, long long v) {
-      __hip_atomic_store(p.host + word, (int64_t)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    };
-    put(7, s_flags);
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the result is complete
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    put(FAT_CHECK_RESULTS + 1, p.ticket);
+    __hip_atomic_store(p.host + FAT_CHECK_RESULTS, (int64_t)INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    finish(7, s_flags);
   }
 }
 
@@ -522,10 +561,8 @@ __global__ __launch_bounds__(kListThreads) void check_lists_kernel(const CheckPa
 namespace {
 
 int check_groups(const fat_check_args* a) {
-  if (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_APPEND || a->kind == FAT_CHECK_COPY ||
-      a->kind == FAT_CHECK_FORK)
-    return 1;
-  if (a->kind == FAT_CHECK_SHARED || a->kind == FAT_CHECK_FREE) {
+  if (a->kind == FAT_CHECK_VARLEN || a->kind == FAT_CHECK_APPEND || a->kind == FAT_CHECK_COPY) return 1;
+  if (a->kind == FAT_CHECK_SHARED || a->kind == FAT_CHECK_FREE || a->kind == FAT_CHECK_FORK) {
     const int64_t n = ((int64_t)a->batch * a->max_pages + fat::kRowsEntries - 1) / fat::kRowsEntries;
     return (int)std::min<int64_t>(1 + std::max<int64_t>(n, 1), FAT_CHECK_MAX_GROUPS);
   }
@@ -652,6 +689,7 @@ extern "C" int fat_check_wait(const fat_check_args* a, void* stream_ptr, int64_t
     result[7] |= 8;
     lo = 0;
   }
+  if (a->kind == FAT_CHECK_FORK && lo == INT_MIN) result[7] |= 512;
   result[12] = lo;
   result[13] = hi;
   result[14] = result[15] = 0;

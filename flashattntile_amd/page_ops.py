@@ -118,6 +118,7 @@ def _fork_flags(flags: int, cache: PagedKVCache) -> None:
     _require(not flags & 64, f"page_table maps a parent's last page outside [0, {pages})")
     _require(not flags & 128, f"pages holds a page outside [0, {pages})")
     _require(not flags & 256, "pages holds a page twice")
+    _require(not flags & 512, "pages holds a page that a row uses")
 
 
 def _outside(t: torch.Tensor, limit: int) -> bool:
@@ -180,7 +181,8 @@ def fork_sequences(cache: PagedKVCache, parents: torch.Tensor, children: torch.T
     length is no multiple of ``page_size``, the child's last page is
     ``pages[i]``, into which the parent's is copied (K and V, and the 8-bit copy
     and scales where given); ``pages[i]`` isn't used where it is one.
-    ``pages`` are pages that no row uses, such as :func:`free_sequences` lists.
+    ``pages`` are pages that no row's tokens use, such as :func:`free_sequences`
+    lists (not one that another row holds ahead, which this call can't see).
     Children must be empty rows and no child a parent; a parent may have any
     number of children.  Table columns behind the child's last page stay as they
     are.  ``page_table`` and ``seq_lens`` are updated in place, on the device.
@@ -228,7 +230,9 @@ def _fork_torch(cache, parents, children, pages, copy, scales) -> None:
     fresh = pages[tail]
     last = cache.page_table[par[tail], full[tail]]
     flags = 64 * _outside(last, pool) | 128 * _outside(fresh, pool)
-    _fork_flags(flags | 256 * (torch.unique(fresh).numel() < fresh.numel()), cache)
+    _fork_flags(flags, cache)  # the rest reads the pages' use
+    flags = 256 * (torch.unique(fresh).numel() < fresh.numel())
+    _fork_flags(flags | 512 * bool(_used_torch(cache, None)[1][fresh.long()].any()), cache)
     rows = cache.page_table[par]
     rows[tail, full[tail]] = fresh
     column = torch.arange(cache.max_pages_per_seq, device=rows.device)

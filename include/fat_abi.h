@@ -53,7 +53,8 @@
 extern "C" {
 #endif
 
-/* 20: FAT_CHECK_COPY and FAT_CHECK_FORK need no scratch memory.
+/* 21: FAT_CHECK_FORK looks at all rows (512).
+ * 20: FAT_CHECK_COPY and FAT_CHECK_FORK need no scratch memory.
  * 19: fat_paged_decode_shared and FAT_CHECK_SHARED.
  * 18: operations on pages (fat_copy_pages, fat_fork_sequences,
  *     fat_free_sequences, fat_compact_pages) and FAT_CHECK_COPY, _FORK, _FREE.
@@ -79,7 +80,7 @@ extern "C" {
  * 8: fp32 decode, any page size and head_dim 32/256 through the generic
  *    decode kernel (FAT_KERNEL_DECODE_GENERIC); the paged prefill `rows`
  *    field replaces the library's environment overrides. */
-#define FAT_ABI_VERSION 20
+#define FAT_ABI_VERSION 21
 
 /* Element types understood by the kernels. */
 enum fat_dtype {
@@ -740,7 +741,7 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *                          (flashattn_tile/quant.py:128-142, the scale range)
  *        FAT_CHECK_COPY    src = ids[0] and dst = ids[1], `count` pages each
  *        FAT_CHECK_FORK    parents, children and pages = ids[0 .. 2], `count`
- *                          each, with seq_lens and the page table
+ *                          each, with seq_lens and the columns that each row uses
  *        FAT_CHECK_FREE    seq_lens, the columns that each row uses, and rows =
  *                          ids[0], `count` >= 0 of them
  *        FAT_CHECK_SHARED  seq_lens, the columns that each row uses, and the groups cu_q [count + 1] with
@@ -771,14 +772,15 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *          child that is a parent too, 16 a child that holds tokens, 32 a
  *          parent longer than the table or negative, and of parents that end
  *          inside a page: 64 that page, 128 pages[i] out of [0, num_pages),
- *          256 pages[i] given twice; SHARED: 1 cu_q decreases, 2 a negative
- *          prefix, 4 one beyond seq_lens - tokens + 1 of a sequence of its
- *          group, 8 a sequence whose table row names other pages than the
- *          group's first where the prefix fills pages.  SHARED also: 3, 4
- *          cu_q[0], cu_q[count]; 5 the most sequences of a group; 6 the longest
- *          prefix (of a group with sequences); 8 the most keys behind the prefix;
- *          9 sum over groups of prefix; 10 sum over sequences of the keys behind
- *          it; 11 sum over groups of prefix x sequences
+ *          256 pages[i] given twice, 512 pages[i] in a column that a row uses;
+ *          SHARED: 1 cu_q decreases, 2 a negative prefix, 4 one beyond
+ *          seq_lens - tokens + 1 of a sequence of its group, 8 a sequence whose
+ *          table row names other pages than the group's first where the prefix
+ *          fills pages.  SHARED also: 3, 4 cu_q[0], cu_q[count]; 5 the most
+ *          sequences of a group; 6 the longest prefix (of a group with
+ *          sequences); 8 the most keys behind the prefix; 9 sum over groups of
+ *          prefix; 10 sum over sequences of the keys behind it; 11 sum over
+ *          groups of prefix x sequences
  * Entries that a kind doesn't name are undefined.
  */
 enum fat_check_kind {
