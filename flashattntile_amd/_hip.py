@@ -472,6 +472,7 @@ class CheckArgs(ctypes.Structure):
         ("ids", _c_vp * 3),
         ("num_pages", _c_i32),
         ("tokens", _c_i32),
+        ("held", _c_vp),
     ]
 
 
@@ -604,7 +605,7 @@ class Check:
 
     def begin(self, kind: int, batch: int, stream: int, cu_q: torch.Tensor | None, cu_k: torch.Tensor | None,
               seq_lens: torch.Tensor | None, page_table: torch.Tensor | None, page_size: int, ids=(),
-              num_pages: int = 0, tokens: int = 1) -> None:
+              num_pages: int = 0, tokens: int = 1, held: torch.Tensor | None = None) -> None:
         if self._pending:
             torch.cuda.synchronize(self._device)
         a = self._args
@@ -616,6 +617,7 @@ class Check:
                 a.ids[i] = t.data_ptr()
             a.num_pages = num_pages
             a.tokens = tokens
+        a.held = None if held is None else held.data_ptr()
         a.cu_q = None if cu_q is None else cu_q.data_ptr()
         a.cu_k = None if cu_k is None else cu_k.data_ptr()
         if seq_lens is not None:
@@ -680,7 +682,7 @@ def float_range(values: torch.Tensor) -> tuple[float, float]:
 def check_begin(kind: int, stream: int, device: torch.device, cu_q: torch.Tensor | None = None,
                 cu_k: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None,
                 page_table: torch.Tensor | None = None, page_size: int = 0, ids=(),
-                num_pages: int = 0, tokens: int = 1) -> Check:
+                num_pages: int = 0, tokens: int = 1, held: torch.Tensor | None = None) -> Check:
     """Begin a check on ``stream``: ``cu_q`` / ``cu_k`` int32 [B + 1],
     ``seq_lens`` int32 [B] (contiguous), ``page_table`` int32 [B, M > 0] with
     a unit column stride, B > 0, on one ROCm device; ``ids``: the int32 lists
@@ -688,7 +690,7 @@ def check_begin(kind: int, stream: int, device: torch.device, cu_q: torch.Tensor
     a shared-prefix decode, with its ``tokens`` per sequence."""
     check = _thread_check(device)
     batch = seq_lens.shape[0] if seq_lens is not None else cu_q.shape[0] - 1 if cu_q is not None else 0
-    check.begin(kind, batch, stream, cu_q, cu_k, seq_lens, page_table, page_size, ids, num_pages, tokens)
+    check.begin(kind, batch, stream, cu_q, cu_k, seq_lens, page_table, page_size, ids, num_pages, tokens, held)
     return check
 
 

@@ -121,6 +121,7 @@ struct CheckParams {
   const int32_t* ids[3];
   int32_t num_pages;
   int32_t tokens;
+  const int32_t* held;
 };
 
 struct RMin { template <typename T> static __device__ __forceinline__ T f(T a, T b) { return a < b ? a : b; } };
@@ -370,6 +371,9 @@ __global__ __launch_bounds__(kRowsThreads) void check_rows_kernel(const CheckPar
         x[1] = max(x[1], len);
         x[2] += pages_of((int)len);
       }
+      if (p.held) {
+        for (int b = tid; b < p.B; b += kRowsThreads) x[3] |= p.held[b] > p.max_pages ? 2 : 0;
+      }
       for (int64_t i = tid; i < p.count; i += kRowsThreads) x[3] |= (unsigned)p.ids[0][i] >= (unsigned)p.B ? 1 : 0;
       const long long r = rows_reduce(x, op, (int)min((max((int64_t)p.B, p.count) + 63) / 64, (int64_t)kRowsWaves));
 #pragma unroll
@@ -387,7 +391,7 @@ __global__ __launch_bounds__(kRowsThreads) void check_rows_kernel(const CheckPar
       const int b = (int)(u / per_row);
       const int32_t* row = p.pt + b * p.pt_sb;
       const int32_t* first = row;
-      const int cols = min(pages_of(p.lens[b]), p.max_pages);
+      int cols = min(pages_of(p.lens[b]), p.max_pages);
       int same = 0;
       if constexpr (SHARED) {
         // The largest g with cu_q[g] <= b, if any: 64 samples at a time.
@@ -404,6 +408,9 @@ __global__ __launch_bounds__(kRowsThreads) void check_rows_kernel(const CheckPar
         const int lead = g < 0 ? b : max(p.cu_q[g], 0);
         same = lead == b ? 0 : min(max(prefix[g], 0) / p.P, cols);
         first = p.pt + lead * p.pt_sb;
+      }
+      if constexpr (!SHARED) {
+        if (p.held) cols = min(max(cols, p.held[b]), p.max_pages);
       }
       const int stride = per_row * 64;
 #pragma unroll 8
@@ -614,7 +621,7 @@ extern "C" int fat_check_begin(const fat_check_args* a, void* stream_ptr) {
   }
   const fat::CheckParams prm{a->cu_q, a->cu_k, a->seq_lens, a->page_table, a->page_table_stride, a->host,
                              a->ticket, a->batch, a->max_pages, a->page_size, a->values, a->count,
-                             {a->ids[0], a->ids[1], a->ids[2]}, a->num_pages, a->tokens};
+                             {a->ids[0], a->ids[1], a->ids[2]}, a->num_pages, a->tokens, a->held};
   const dim3 grid((unsigned)check_groups(a)), block(fat::kCheckThreads);
   switch (a->kind) {
     case FAT_CHECK_CACHE: hipLaunchKernelGGL((fat::check_kernel<FAT_CHECK_CACHE>), grid, block, 0, stream, prm); break;

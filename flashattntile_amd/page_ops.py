@@ -257,13 +257,30 @@ def _used_torch(cache: PagedKVCache, held: torch.Tensor | None) -> tuple[torch.T
     return columns, used
 
 
-def _used_stats(cache: PagedKVCache) -> tuple[int, int, int, int]:
-    """Min and max length, and min and max page id of the columns that each row's
-    tokens use (0, -1 where none does)."""
+def _assess_used(cache: PagedKVCache, held: torch.Tensor | None, stats: tuple[int, int, int, int],
+                 beyond: bool) -> None:
+    """The checks of lengths, ``held`` and the columns that rows use, on their numbers."""
+    _require(not beyond, f"held counts more columns than the page table has ({cache.max_pages_per_seq})")
+    _assess_cache(cache, stats, check_pages=held is None)
+    if held is not None:  # pages may be held where no row has tokens
+        lo, hi = stats[2:]
+        _require(lo >= 0, "page_table contains a negative page id")
+        _require(hi < cache.num_pages, f"page_table references page {hi} but cache has {cache.num_pages} pages")
+
+
+def _beyond(cache: PagedKVCache, held: torch.Tensor | None) -> bool:
+    return held is not None and bool((held > cache.max_pages_per_seq).any())
+
+
+def _used_stats(cache: PagedKVCache, held: torch.Tensor | None) -> tuple[int, int, int, int]:
+    """Min and max length, and min and max page id of the columns that rows use
+    (0, -1 where none does)."""
     lens = cache.seq_lens.long()
     if not lens.numel():
         return 0, 0, 0, -1
     n = torch.div(lens.clamp_min(0) + cache.page_size - 1, cache.page_size, rounding_mode="floor")
+    if held is not None:
+        n = torch.maximum(n, held.long())
     ids = cache.page_table[torch.arange(cache.page_table.shape[1], device=n.device) < n[:, None]]
     return (int(lens.min()), int(lens.max())) + ((int(ids.min()), int(ids.max())) if ids.numel() else (0, -1))
 
@@ -284,7 +301,7 @@ def free_sequences(cache: PagedKVCache, rows: torch.Tensor, *, held: torch.Tenso
     dev = cache.k_cache.device
     if not cache.k_cache.is_cuda or not cache.page_table.numel() or not cache.num_pages:
         _require(not _outside(rows, cache.batch_size), f"rows holds a row outside [0, {cache.batch_size})")
-        _assess_cache(cache, _used_stats(cache))
+        _assess_used(cache, held, _used_stats(cache, held), _beyond(cache, held))
         cache.seq_lens[rows.long()] = 0
         if held is not None:
             held[rows.long()] = 0
@@ -301,7 +318,8 @@ def free_sequences(cache: PagedKVCache, rows: torch.Tensor, *, held: torch.Tenso
         check = None
         if validate:
             check = _hip.check_begin(_hip.CHECK_FREE, stream, dev, seq_lens=cache.seq_lens,
-                                     page_table=cache.page_table, page_size=cache.page_size, ids=(rows,))
+                                     page_table=cache.page_table, page_size=cache.page_size, ids=(rows,),
+                                     held=held)
         # prepared while the check kernel runs
         pages = torch.empty(cache.num_pages, dtype=torch.int32, device=dev)
         count = torch.empty((), dtype=torch.int32, device=dev)
@@ -309,7 +327,7 @@ def free_sequences(cache: PagedKVCache, rows: torch.Tensor, *, held: torch.Tenso
         args = _hip.free_args(cache, rows, held, pages, count, workspace)
         if check is not None:
             r = check.wait()
-            _assess_cache(cache, _stats_of(r))
+            _assess_used(cache, held, _stats_of(r), bool(r[7] & 2))
             _require(not r[7] & 1, f"rows holds a row outside [0, {cache.batch_size})")
         _hip.page_operation("fat_free_sequences", args, stream)
     return pages, count
@@ -342,7 +360,7 @@ def compact_pages(cache: PagedKVCache, *, held: torch.Tensor | None = None, quan
     held = _held(cache, held, written=False)
     dev = cache.k_cache.device
     if not cache.k_cache.is_cuda or not cache.page_table.numel() or not cache.num_pages:
-        _assess_cache(cache, _used_stats(cache))
+        _assess_used(cache, held, _used_stats(cache, held), _beyond(cache, held))
         columns, used = _used_torch(cache, held)
         n = int(used.sum())
         ids = torch.arange(cache.num_pages, device=dev)
@@ -363,13 +381,14 @@ def compact_pages(cache: PagedKVCache, *, held: torch.Tensor | None = None, quan
         check = None
         if validate:
             check = _hip.check_begin(_hip.CHECK_FREE, stream, dev, seq_lens=cache.seq_lens,
-                                     page_table=cache.page_table, page_size=cache.page_size)
+                                     page_table=cache.page_table, page_size=cache.page_size, held=held)
         # prepared while the check kernel runs
         remap = torch.empty(cache.num_pages, dtype=torch.int32, device=dev)
         count = torch.empty((), dtype=torch.int32, device=dev)
         workspace = _hip.pages_workspace(cache.num_pages, dev)
         args = _hip.compact_args(cache, held, remap, count, workspace, copy, scales)
         if check is not None:
-            _assess_cache(cache, _stats_of(check.wait()))
+            r = check.wait()
+            _assess_used(cache, held, _stats_of(r), bool(r[7] & 2))
         _hip.page_operation("fat_compact_pages", args, stream)
     return remap, count

@@ -53,7 +53,7 @@
 extern "C" {
 #endif
 
-/* 21: FAT_CHECK_FORK looks at all rows (512).
+/* 21: FAT_CHECK_FORK looks at all rows (512); FAT_CHECK_FREE at held.
  * 20: FAT_CHECK_COPY and FAT_CHECK_FORK need no scratch memory.
  * 19: fat_paged_decode_shared and FAT_CHECK_SHARED.
  * 18: operations on pages (fat_copy_pages, fat_fork_sequences,
@@ -742,8 +742,8 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *        FAT_CHECK_COPY    src = ids[0] and dst = ids[1], `count` pages each
  *        FAT_CHECK_FORK    parents, children and pages = ids[0 .. 2], `count`
  *                          each, with seq_lens and the columns that each row uses
- *        FAT_CHECK_FREE    seq_lens, the columns that each row uses, and rows =
- *                          ids[0], `count` >= 0 of them
+ *        FAT_CHECK_FREE    seq_lens, held (optional), the columns that each row
+ *                          uses or holds, and rows = ids[0], `count` >= 0 of them
  *        FAT_CHECK_SHARED  seq_lens, the columns that each row uses, and the groups cu_q [count + 1] with
  *                          the prefixes ids[0] [count]; tokens = queries per
  *                          sequence
@@ -763,16 +763,18 @@ int fat_cache_stats(const fat_cache_stats_args* args, void* stream);
  *   12, 13 min and max page id: over every row and the columns below
  *          ceil(max(seq_lens) / page_size) (CACHE, PAGED; INT32_MAX and
  *          INT32_MIN when no column is used), of the columns c < ceil(seq_lens[b] /
- *          page_size) of each row (FREE, SHARED; likewise), or of the entries
+ *          page_size) of each row, with held those c < held[b] too (FREE, SHARED;
+ *          likewise), or of the entries
  *          [b, clamp(floor(seq_lens[b] / page_size), 0, max_pages - 1)] (APPEND);
  *          the bits of the fp32 min and max, NaN if a value is (RANGE)
  *   7      COPY: 1 a src, 2 a dst out of [0, num_pages), 4 a dst given twice, 8
- *          a dst that is a src too; FREE: 1 a row out of [0, batch); FORK: 1 a
- *          parent, 2 a child out of [0, batch), 4 a child given twice, 8 a
- *          child that is a parent too, 16 a child that holds tokens, 32 a
- *          parent longer than the table or negative, and of parents that end
- *          inside a page: 64 that page, 128 pages[i] out of [0, num_pages),
- *          256 pages[i] given twice, 512 pages[i] in a column that a row uses;
+ *          a dst that is a src too; FREE: 1 a row out of [0, batch), 2 a held
+ *          beyond max_pages; FORK: 1 a parent, 2 a child out of [0, batch), 4 a
+ *          child given twice, 8 a child that is a parent too, 16 a child that
+ *          holds tokens, 32 a parent longer than the table or negative, and of
+ *          parents that end inside a page: 64 that page, 128 pages[i] out of
+ *          [0, num_pages), 256 pages[i] given twice, 512 pages[i] in a column
+ *          that a row uses;
  *          SHARED: 1 cu_q decreases, 2 a negative prefix, 4 one beyond
  *          seq_lens - tokens + 1 of a sequence of its group, 8 a sequence whose
  *          table row names other pages than the group's first where the prefix
@@ -814,6 +816,7 @@ typedef struct fat_check_args {
   const int32_t* ids[3]; /* [count] each: COPY, FORK, FREE and SHARED only */
   int32_t num_pages; /* COPY and FORK only */
   int32_t tokens;    /* SHARED only */
+  const int32_t* held; /* [batch] or NULL: FREE only */
 } fat_check_args;
 
 /* Enqueue the check on `stream`.  FAT_E_LAUNCH while the stream is capturing

@@ -8,7 +8,7 @@ import torch
 
 from test_page_ops import _cache, _ids, _same, _snapshot, device
 
-from flashattntile_amd import PagedKVCache, fork_sequences
+from flashattntile_amd import PagedKVCache, compact_pages, fork_sequences, free_sequences
 
 
 def _state(cache):
@@ -105,3 +105,69 @@ def test_fork_looks_at_every_column_of_large_tables(dev, rows, width, pages):
             cache.seq_lens[where[0]] = P * where[1]  # and now just not
             call()
             assert int(cache.seq_lens[rows]) == 3
+
+
+# ---------------------------------------------------------------------------
+# held
+# ---------------------------------------------------------------------------
+@device
+@pytest.mark.parametrize("name", ["free", "compact"])
+def test_held_columns_are_checked(dev, name):
+    """Columns that only `held` covers name pages too, and are columns of the table."""
+    def run(cache, held):
+        if name == "free":
+            return free_sequences(cache, _ids([0], dev), held=held)
+        return compact_pages(cache, held=held)
+
+    lens = [20, 40, 0, 1]
+    for row, column, value, error in ((2, 3, 1 << 20, "references page 1048576"), (0, 4, -3, "negative page id"),
+                                      (3, 1, None, "references page"), (2, 0, -1, "negative page id")):
+        cache = _cache(lens, 16, dev=dev, spare=8, width=5)
+        cache.page_table[row, column] = cache.num_pages if value is None else value
+        held = _ids([5, 3, 4, 2], dev)
+        before = _snapshot(cache), _state(cache)
+        with pytest.raises(AssertionError, match=error):
+            run(cache, held)
+        _same(_snapshot(cache), before[0])
+        assert _state(cache) == before[1] and held.tolist() == [5, 3, 4, 2]
+        held[row] = column  # the columns before it
+        run(cache, held)
+    for many in (6, 2 ** 31 - 1):
+        cache = _cache(lens, 16, dev=dev, spare=8, width=5)
+        before = _snapshot(cache), _state(cache)
+        with pytest.raises(AssertionError, match="held counts more columns than the page table has \\(5\\)"):
+            run(cache, _ids([0, many, 0, 0], dev))
+        _same(_snapshot(cache), before[0])
+        assert _state(cache) == before[1]
+        run(cache, _ids([0, 5, -1, -2 ** 31], dev))  # less than its tokens' columns: those
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width", [(40, 3000), (3000, 40), (5000, 3)])
+def test_held_columns_of_large_tables_are_checked(rows, width):
+    print(f"held {rows} {width}", flush=True)
+    k = torch.zeros(50, 2, 1, 2, device="cuda")
+    for where in ((rows - 1, width - 1), (0, 0), (rows // 2, width // 2)):
+        table = torch.zeros(rows, width, dtype=torch.int32, device="cuda")
+        table[where] = 50
+        cache = PagedKVCache(k, k.clone(), table, torch.zeros(rows, dtype=torch.int32, device="cuda"), 2)
+        held = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        held[where[0]] = where[1] + 1
+        with pytest.raises(AssertionError, match="references page 50"):
+            free_sequences(cache, _ids([], "cuda"), held=held)
+        with pytest.raises(AssertionError, match="references page 50"):
+            compact_pages(cache, held=held)
+        held[where[0]] = where[1]
+        pages, count = free_sequences(cache, _ids([], "cuda"), held=held)
+        assert int(count) == (49 if where[1] else 50)
+
+
+@pytest.mark.gpu
+def test_held_of_one_call_is_not_the_next_one_s():
+    """On one device and thread the checks share a block of arguments."""
+    cache = _cache([20, 40, 0, 1], 16, dev="cuda", spare=8, width=5)
+    cache.page_table[2, 3] = -1
+    for call in (free_sequences, lambda c, rows, **more: compact_pages(c, **more)):
+        with pytest.raises(AssertionError, match="negative page id"):
+            call(cache, _ids([], "cuda"), held=_ids([0, 0, 4, 0], "cuda"))
+        call(cache, _ids([], "cuda"))
