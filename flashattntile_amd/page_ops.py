@@ -50,6 +50,9 @@ def _parts(cache: PagedKVCache, quantized, scales, shared_table: bool):
         _require(not _eight_bit(cache.k_cache.dtype), "an int8/float8 cache has no 8-bit copy")
         copy = _quant_pair(cache, quantized)
         _require(copy[2].stride() == copy[3].stride(), "k and v scales must share strides")
+        if cache.k_cache.is_cuda:
+            _require(copy[0].stride(3) == 1 and copy[1].stride(3) == 1,
+                     "the head_dim axis of the quantised pages must be contiguous")
         qcache = quantized[0]
         if shared_table:
             for name in ("page_table", "seq_lens"):

@@ -6,9 +6,9 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_page_ops import _cache, _ids, _same, _snapshot, device
+from test_page_ops import _cache, _ids, _mirror, _same, _snapshot, device
 
-from flashattntile_amd import PagedKVCache, compact_pages, fork_sequences, free_sequences
+from flashattntile_amd import PagedKVCache, compact_pages, copy_pages, fork_sequences, free_sequences
 
 
 def _state(cache):
@@ -171,3 +171,32 @@ def test_held_of_one_call_is_not_the_next_one_s():
         with pytest.raises(AssertionError, match="negative page id"):
             call(cache, _ids([], "cuda"), held=_ids([0, 0, 4, 0], "cuda"))
         call(cache, _ids([], "cuda"))
+
+
+# ---------------------------------------------------------------------------
+# The 8-bit copy's layout
+# ---------------------------------------------------------------------------
+@device
+@pytest.mark.parametrize("name", ["copy", "fork", "compact"])
+@pytest.mark.parametrize("spread", ["k_cache", "v_cache"])
+def test_an_8_bit_copy_whose_rows_are_not_contiguous(dev, name, spread):
+    """The kernels read head_dim with a unit stride: refused on the GPU, as append_tokens does."""
+    cache = _cache([21, 5, 32, 0], 16, dtype=torch.bfloat16, dev=dev, spare=30)
+    copy, scales = _mirror(cache)
+    wide = torch.zeros(*copy.k_cache.shape, 2, dtype=torch.int8, device=dev)
+    wide[..., 0] = getattr(copy, spread)
+    setattr(copy, spread, wide[..., 0])
+    used = set(cache.page_table.flatten().tolist())
+    fresh = [p for p in range(cache.num_pages) if p not in used]
+    call = {"copy": lambda: copy_pages(cache, _ids([0], dev), _ids([fresh[0]], dev), quantized=(copy, scales)),
+            "fork": lambda: fork_sequences(cache, _ids([0], dev), _ids([3], dev), _ids([fresh[0]], dev),
+                                           quantized=(copy, scales)),
+            "compact": lambda: compact_pages(cache, quantized=(copy, scales))}[name]
+    before = _snapshot(cache, (copy, scales)), _state(cache)
+    if dev == "cpu":
+        call()  # torch takes any strides
+        return
+    with pytest.raises(AssertionError, match="head_dim axis of the quantised pages must be contiguous"):
+        call()
+    _same(_snapshot(cache, (copy, scales)), before[0])
+    assert _state(cache) == before[1]
