@@ -708,15 +708,11 @@ extern "C" int fat_fork_sequences(const fat_fork_args* a, void* stream_ptr) {
                         a->count, a->batch, a->max_pages, (long long)a->page_table_stride);
     return FAT_E_INVALID;
   }
-  // More forks than rows give some row twice; and a grid is at most 65535 high.
-  if (a->count > a->batch || a->count > 65535) {
-    fat_host::set_error("fat_fork_sequences: at most min(batch, 65535) forks in a call, got %d", a->count);
+  if (a->count > a->batch) {  // some row would be given twice
+    fat_host::set_error("fat_fork_sequences: at most batch = %d forks in a call, got %d", a->batch, a->count);
     return FAT_E_INVALID;
   }
   if (a->count == 0) return FAT_OK;
-  prm.parents = a->parents;
-  prm.children = a->children;
-  prm.pages = a->pages;
   prm.pt = a->page_table;
   prm.lens = a->seq_lens;
   prm.pt_sb = a->page_table_stride;
@@ -724,10 +720,18 @@ extern "C" int fat_fork_sequences(const fat_fork_args* a, void* stream_ptr) {
   prm.max_pages = a->max_pages;
   prm.P = a->pool.page_size;
   const unsigned table = (unsigned)std::min<int64_t>((a->max_pages + 1023) / 1024, 64);
-  const dim3 grid(std::max(copy_grid(prm.planes, 1), table), (unsigned)a->count, prm.planes.n + 1);
   hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
-  hipLaunchKernelGGL(fat::fork_kernel, grid, dim3(fat::kCopyThreads), 0, stream, prm);
-  return fat_host::launch_status("fork_kernel");
+  constexpr int kHeight = 65535;  // of a grid; the forks of a call are independent
+  for (int64_t i = 0; i < a->count && rc == FAT_OK; i += kHeight) {
+    prm.parents = a->parents + i;
+    prm.children = a->children + i;
+    prm.pages = a->pages + i;
+    const dim3 grid(std::max(copy_grid(prm.planes, 1), table), (unsigned)std::min<int64_t>(a->count - i, kHeight),
+                    prm.planes.n + 1);
+    hipLaunchKernelGGL(fat::fork_kernel, grid, dim3(fat::kCopyThreads), 0, stream, prm);
+    rc = fat_host::launch_status("fork_kernel");
+  }
+  return rc;
 }
 
 extern "C" int fat_free_sequences(const fat_free_args* a, void* stream_ptr) {
