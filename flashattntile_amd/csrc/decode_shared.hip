@@ -838,6 +838,12 @@ extern "C" int fat_paged_decode_shared(const fat_shared_args* a, void* stream_pt
   }
   const int T = a->q_len > 1 ? a->q_len : 1;
   const int eb = kv == fat::KV_SAME ? 2 : 1;
+  // Rows of a KV head are numbered in 32 bits, 128 a tile.
+  if ((int64_t)a->batch * T > (0x7fffffffLL - 128) / (a->num_heads / a->num_kv_heads)) {
+    fat_host::set_error("fat_paged_decode_shared: batch %d x q_len %d x %d heads per KV head are too many query rows",
+                        a->batch, T, a->num_heads / a->num_kv_heads);
+    return FAT_E_UNSUPPORTED;
+  }
   const uintptr_t align = (uintptr_t)a->q | (uintptr_t)(2 * a->q_stride_b) | (uintptr_t)(2 * a->q_stride_h) |
                           (uintptr_t)(T > 1 ? 2 * a->q_stride_t : 0) | (uintptr_t)a->workspace | (uintptr_t)a->k_cache |
                           (uintptr_t)a->v_cache | (uintptr_t)(eb * a->k_stride_page) |

@@ -79,3 +79,16 @@ def test_a_workspace_on_top_of_the_scales():
 ])
 def test_refusals(more, code, error):
     _refused(_args(**more), code, error)
+
+
+@pytest.mark.parametrize("batch,q_len,heads,kv_heads,code,error", [
+    # batch x q_len = 2^31: the rows, and with them the bytes of workspace, were counted in 32 bits
+    (1 << 25, 64, 1, 1, UNSUPPORTED, "query rows"), (1 << 30, 2, 1, 1, UNSUPPORTED, "query rows"),
+    (2 ** 31 - 1, 64, 1, 1, UNSUPPORTED, "query rows"),
+    # 2^31 rows of one KV head
+    (1 << 24, 1, 128, 1, UNSUPPORTED, "query rows"), (1 << 20, 64, 64, 2, UNSUPPORTED, "query rows"),
+    # 2^30 rows: their workspace is what is missing
+    (1 << 24, 64, 1, 1, INVALID, "bytes of workspace"), (1 << 24, 1, 64, 1, INVALID, "bytes of workspace"),
+])
+def test_rows_beyond_32_bits(batch, q_len, heads, kv_heads, code, error):
+    _refused(_args(batch=batch, max_group=1, q_len=q_len, num_heads=heads, num_kv_heads=kv_heads), code, error)
