@@ -230,12 +230,20 @@ def paged_decode_shared_launch(q: torch.Tensor, cache: PagedKVCache, cu_groups: 
     batch): the outputs of those beyond are undefined.  Lengths, table, groups
     and prefixes are read on the device at every run.
     ``q`` must be contiguous and begin on a 16-byte boundary (else it is copied);
-    ``out`` and ``workspace`` (uint8, 4 x rows x heads x partials x (head_dim + 2)
-    bytes) may be passed in to avoid allocations.
+    ``out`` (of ``q``'s shape, dtype and device, head_dim contiguous) and
+    ``workspace`` (contiguous, 4 x rows x heads x partials x (head_dim + 2) bytes; a
+    smaller one is left aside) may be passed in to avoid allocations; launches that
+    may run at the same time, replays of two graphs among them, need a workspace each.
     Takes fp16/bf16 queries at head_dim 64 or 128, else raises.
     """
     with _hip.on_device(q.device):
         q = _dense_query(q)
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
+                                or out.stride(-1) != 1):
+            raise ValueError(f"out must be a {q.dtype} tensor of q's shape {tuple(q.shape)} on its device, head_dim "
+                             f"contiguous")
+        if workspace is not None and (workspace.device != q.device or not workspace.is_contiguous()):
+            raise ValueError("workspace must be a contiguous tensor on q's device")
         cache, cu_groups, prefix_lens = _dense(cache, cu_groups, prefix_lens)
         a, out, _keep = _block(q, cache, cu_groups, prefix_lens, softmax_scale, scales, out)
         cfg = _resolve(config, q, cache, max_prefix, max_own, max_group or q.shape[0], prefix_lens.shape[0],
