@@ -713,19 +713,28 @@ __global__ __launch_bounds__(64 * kJoinRows) void shared_join_kernel(const Share
 #pragma unroll
   for (int e = 0; e < E; ++e) a[e] = 0.f;
   const float* acc = p.ws_acc + row * S * D + E * lane;
-  // Eight slots' loads in flight; those of weight 0 may never have been written.
-  for (int s0 = 0; s0 < S; s0 += 8) {
-    float x[8][E];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[i][e] = acc[(int64_t)min(s0 + i, S - 1) * D + e];
+  // Eight slots' loads in flight.  Those of weight 0 are left out: they may never have
+  // been written, and few of a batch's sequences have keys in all of their slots.
+  unsigned long long left[2] = {__ballot(f[0] != 0.f), __ballot(f[1] != 0.f)};
+  while (left[0] | left[1]) {  // uniform
+    float x[8][E], w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int s = s0 + i;
-      const float w = __shfl(s < 64 ? f[0] : f[1], s & 63);  // 0 for s >= S
+      const bool low = left[0] != 0;
+      const unsigned long long some = low ? left[0] : left[1];
+      const int at = some ? __builtin_ctzll(some) : 0;
+      // None left: slot 0 or 64 once more, with a weight of 0.
+      w[i] = some ? __shfl(low ? f[0] : f[1], at) : 0.f;
+      const int s = min(at + (low ? 0 : 64), S - 1);
 #pragma unroll
-      for (int e = 0; e < E; ++e) a[e] = __builtin_fmaf(w != 0.f ? x[i][e] : 0.f, w, a[e]);
+      for (int e = 0; e < E; ++e) x[i][e] = acc[(int64_t)s * D + e];
+      if (low) left[0] &= left[0] - 1;
+      else left[1] &= left[1] - 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) a[e] = __builtin_fmaf(w[i] != 0.f ? x[i][e] : 0.f, w[i], a[e]);
     }
   }
   const int64_t bt = row / p.H;

@@ -141,7 +141,7 @@ def _up(n: int, to: int) -> int:
 
 
 def shared_splits(num_kv_heads: int, group_rows: int, own_tiles: int, groups: float, max_prefix: int,
-                  sequences: float, max_own: int, rows: int) -> dict:
+                  sequences: float, max_own: int, rows: int, batch: int | None = None) -> dict:
     """Partials of a launch: ``prefix_split`` x ``prefix_chunk`` keys of every
     prefix, ``split`` x ``chunk`` own keys of every sequence.
 
@@ -149,7 +149,8 @@ def shared_splits(num_kv_heads: int, group_rows: int, own_tiles: int, groups: fl
     32-row tiles of a sequence; ``rows``: query rows of all heads.  ``groups`` and
     ``sequences`` count those of the longest's length (the sum of all lengths by the
     longest): splits that fit the longest leave the chip to the others' few
-    workgroups otherwise.
+    workgroups otherwise.  ``batch``: all sequences (default: ``sequences``), whose
+    workgroups a split has too, keys or not.
     """
     # n chunks of K keys cost a chain of a K / n us, and n b for their partials (1040
     # bytes per row, written and read) and workgroups: least at sqrt(a K / b), a little
@@ -162,8 +163,22 @@ def shared_splits(num_kv_heads: int, group_rows: int, own_tiles: int, groups: fl
     best = 0.8 * math.sqrt(per_key * max_prefix / (2.0e-4 * rows + 0.01 * items))
     prefix_split = max(1, min(round(min(best, 256 / items)), 64, max_prefix // 32))
     # Four workgroups of own keys per CU (128 sequences of 100 to 2000 keys on fp8: 1
-    # chunk 66.6 us, 2 60.4, 4 62.7, 8 72.6).
-    split = max(1, min(int(1024 / max(1.0, sequences * num_kv_heads * own_tiles)), 64, max_own // 256))
+    # chunk 66.6 us, 2 60.4, 4 62.7, 8 72.6), and as for prefixes: a chunk costs 1.7 ns
+    # per workgroup, those without keys among them (bf16, one long sequence among short
+    # ones of 100 keys, us at the chunks taken and at 64: 128 sequences, one of 32768
+    # keys, 13: 104, 185; 256 of 4 tokens 9: 190, 355; 256 of 8, one of 65536, 13: 312,
+    # 471).
+    per_slot = num_kv_heads * own_tiles
+    split = max(1, min(int(1024 / max(1.0, sequences * per_slot)), 64, max_own // 256))
+    if split > 1:
+        per_slot *= max(batch or 0, sequences)
+        split = max(1, min(split, round(math.sqrt(0.0092 * max_own / (0.15 + 0.0017 * per_slot)))))
+    # At most 512 MiB of partials, where two slots fit that (520 bytes a row at head_dim
+    # 128; all 128 slots of 8065 rows do).
+    if rows > 8000:
+        slots = 2 ** 29 // (520 * rows)
+        prefix_split = min(prefix_split, max(1, slots - 1))
+        split = min(split, max(1, slots - prefix_split))
     return _chunks(prefix_split, split, max_prefix, max_own)
 
 
@@ -256,7 +271,7 @@ def _resolve(config, q, cache, max_prefix: int, max_own: int, max_group: int, gr
              sequences: float) -> dict:
     per_seq = (q.shape[1] if q.dim() == 4 else 1) * q.shape[-2] // cache.num_kv_heads
     cfg = shared_splits(cache.num_kv_heads, max_group * per_seq, -(-per_seq // 32), groups, max_prefix, sequences,
-                        max_own, q.shape[0] * per_seq * cache.num_kv_heads)
+                        max_own, q.shape[0] * per_seq * cache.num_kv_heads, q.shape[0])
     given = _given(config) if config else None
     if not given:
         return cfg
