@@ -899,10 +899,6 @@ def shared_args(q: torch.Tensor, cache, cu_groups: torch.Tensor, prefix_lens: to
     return a
 
 
-def shared_workspace_bytes(rows: int, num_heads: int, head_dim: int, splits: int) -> int:
-    return int(lib().fat_paged_decode_shared_workspace_bytes(rows, num_heads, head_dim, splits))
-
-
 def shared_with_args(a: SharedArgs, workspace: torch.Tensor, stream: int) -> None:
     """Enqueue ``fat_paged_decode_shared`` with a prepared argument block."""
     a.workspace = _ptr(workspace)

@@ -55,6 +55,35 @@ struct DecodeParams {
 constexpr int kBalMaxSeqs = 1024;
 constexpr int kBalRows = 16;
 
+// 16 bytes of int8 or OCP e4m3 codes as their exact values in fp16 (8 packed
+// pairs).  With fp16 queries the VALU and MFMA decode stage K this way and apply
+// k_scale to the fp32 scores, as the reference's quantised kernel does
+// (kernels/decode.py:419-429: k = float(x) * k_scale, scores in fp32):
+// 5 (int8) or 2 (fp8) instructions per 4 elements instead of 11 or 8 for
+// round_to_fp16(float(x) * scale).  V keeps that per-element dequantisation:
+// folding v_scale into P would round P after a scale that differs per page,
+// and pages whose scales differ by 2^15 or more (two can share a 32-key
+// block) would leave the smaller one's P in fp16's subnormal range.
+template <int KV>
+__device__ __forceinline__ void k8_exact_f16(const u32x4& raw, u32 (&out)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (KV == KV_I8) {
+      // fp16 bits 0x6400 | u are 1024 + u exactly (u = x + 128, the byte with
+      // its sign bit flipped); adding -1152 leaves x.
+      const u32 u = raw[j] ^ 0x80808080u;
+      const f16x2 bias = {(f16)-1152.0f, (f16)-1152.0f};
+      out[2 * j] = __builtin_bit_cast(
+          u32, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias);
+      out[2 * j + 1] = __builtin_bit_cast(
+          u32, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias);
+    } else {  // OCP e4m3 -> fp16 is exact
+      out[2 * j] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[j], 1.0f, false));
+      out[2 * j + 1] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[j], 1.0f, true));
+    }
+  }
+}
+
 }  // namespace fat
 
 namespace fat_host {

@@ -26,9 +26,9 @@
 // Both kinds run the same tile: 32 keys x 32 rows per wave on
 // v_mfma_f32_32x32x16, S^T = K Q^T with K as the A operand (its rows staged in
 // LDS) and O^T += V^T P^T with P^T straight from S^T's registers and V^T by
-// transposed LDS reads.  A workgroup's four waves are RB row blocks x KG = 4 / RB
-// key groups: the RB waves of a key group share its tiles, the key groups take
-// tiles in turn and join at the end.
+// transposed LDS reads.  RB = 4: a workgroup's four waves are four blocks of 32 rows
+// and share every tile.  RB = 1: they have the same 32 rows, take tiles in turn (KG =
+// 4 key groups) and join at the end.
 #include <algorithm>
 
 #include "decode_params.h"
@@ -95,34 +95,28 @@ __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(
 // 16 int8 or e4m3 codes as their exact values in QT (8 packed pairs).
 template <typename QT, int KV>
 __device__ __forceinline__ void codes_exact(const u32x4& raw, u32 (&o)[8]) {
-  constexpr bool H = std::is_same<QT, F16>::value;
+  if constexpr (std::is_same<QT, F16>::value) {
+    k8_exact_f16<KV>(raw, o);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if constexpr (KV == KV_FP8 && H) {
-      o[2 * j] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[j], 1.0f, false));
-      o[2 * j + 1] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[j], 1.0f, true));
-    } else if constexpr (KV == KV_FP8) {
-      o[2 * j] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j], 1.0f, false));
-      o[2 * j + 1] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j], 1.0f, true));
-    } else if constexpr (H) {
-      // fp16 bits 0x6400 | u are 1024 + u exactly (u = x + 128, the byte with its
-      // sign bit flipped); adding -1152 leaves x.
-      const u32 u = raw[j] ^ 0x80808080u;
-      const f16x2 bias = {(f16)-1152.0f, (f16)-1152.0f};
-      o[2 * j] = __builtin_bit_cast(u32, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias);
-      o[2 * j + 1] = __builtin_bit_cast(u32, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias);
-    } else {
-      float f[4];
-      i8x4_biased(raw[j], f);
-      o[2 * j] = Pair<QT>::pack(f[0] - 128.0f, f[1] - 128.0f);
-      o[2 * j + 1] = Pair<QT>::pack(f[2] - 128.0f, f[3] - 128.0f);
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (KV == KV_FP8) {
+        o[2 * j] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j], 1.0f, false));
+        o[2 * j + 1] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j], 1.0f, true));
+      } else {
+        float f[4];
+        i8x4_biased(raw[j], f);
+        o[2 * j] = Pair<QT>::pack(f[0] - 128.0f, f[1] - 128.0f);
+        o[2 * j + 1] = Pair<QT>::pack(f[2] - 128.0f, f[3] - 128.0f);
+      }
     }
   }
 }
 
 template <typename QT, int KV, int D, int RB>
 struct SharedTile {
-  static constexpr int KG = kSharedWaves / RB;
+  static_assert(RB == 1 || RB == kSharedWaves, "one row block, or one per wave");
+  static constexpr int KG = kSharedWaves / RB;  // key groups
   static constexpr int kBufs = RB == 1 ? 1 : 2;  // LDS tiles per key group
   static constexpr int KS = D / 16;              // MFMA k-steps
   static constexpr int DB = D / 32;              // 32-dim blocks of O^T
@@ -161,7 +155,9 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
   constexpr bool FOLD = Tl::FOLD;
   using VT = typename Tl::VT;
   // P enters the second product as bf16 hi + lo parts: one bf16 alone (2^-9) would
-  // show beside the output's own rounding where a row sees few keys.
+  // show beside the output's own rounding where a row sees few keys.  fp16 P is one
+  // part: its half step, 2^-11, is the output's own (relative error 2.6e-4 to 2.9e-4,
+  // with P in 32 bits 2.1e-4), and a second part would double the second product.
   constexpr bool SPLIT_P = std::is_same<VT, BF16>::value;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -239,8 +235,8 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
       ++c;
     }
   };
-  uint32_t last_col = 0, last_slot = 0;
-  if (n_tiles > 0) place((uint32_t)t_end - 1, last_col, last_slot);
+  uint32_t last_col, last_slot;
+  place((uint32_t)t_end - 1, last_col, last_slot);
   last_col = __builtin_amdgcn_readfirstlane(last_col);
   last_slot = __builtin_amdgcn_readfirstlane(last_slot);
 #pragma unroll
@@ -481,78 +477,73 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
     // of tile i beside the maximum of tile i + 1.  K(i + 1) and V(i) lie in LDS, K(i +
     // 2) and V(i + 1) in registers (loaded a round ago, stored at this one's end),
     // and K(i + 3) and V(i + 2) are loaded.  One barrier a round: behind it every wave is
-    // done with round i - 1, whose buffers the round's stores take.  All key groups
-    // run the same number of rounds; tiles behind the end stage the last key, and
-    // their scores are masked.
-    const int rounds = (n_tiles + KG - 1) / KG;
-    if (rounds > 0) {
-      Raw Ra, Rb;
-      f32x16 sa, sb;
-      lookup(kg);
-      advance(kg + KG);
-      fetch_k(Ra);
-      fetch_v(Ra, k_page, k_slot);
-      advance(kg + 2 * KG);
-      fetch_k(Rb);
-      fetch_v(Rb, k_page, k_slot);
-      advance(kg + 3 * KG);
-      store_k(Ra, 0);
-      store_v(Ra, kg, 0);
-      store_k(Rb, 1);
-      fetch_k(Rb);
+    // done with round i - 1, whose buffers the round's stores take.  Tiles behind the
+    // end stage the last key, and their scores are masked.
+    Raw Ra, Rb;
+    f32x16 sa, sb;
+    lookup(0);
+    advance(1);
+    fetch_k(Ra);
+    fetch_v(Ra, k_page, k_slot);
+    advance(2);
+    fetch_k(Rb);
+    fetch_v(Rb, k_page, k_slot);
+    advance(3);
+    store_k(Ra, 0);
+    store_v(Ra, 0, 0);
+    store_k(Rb, 1);
+    fetch_k(Rb);
+    __syncthreads();
+    qk(sa, 0);
+    scale_s(sa, 0);
+    mask(sa, 0);
+    raise(largest(sa));
+    auto round = [&](int i, f32x16& s, f32x16& s2, const Raw& X, Raw& Y) __attribute__((always_inline)) {
+      const int now = i & 1, next = now ^ 1;
+      advance(i + 4);
+      fetch_v(Y, v_page, v_slot);
+      fetch_k(Y);
       __syncthreads();
-      qk(sa, 0);
-      scale_s(sa, 0);
-      mask(sa, kg);
-      raise(largest(sa));
-      auto round = [&](int i, f32x16& s, f32x16& s2, const Raw& X, Raw& Y) __attribute__((always_inline)) {
-        const int t = kg + i * KG;
-        const int now = i & 1, next = now ^ 1;
-        advance(t + 4 * KG);
-        fetch_v(Y, v_page, v_slot);
-        fetch_k(Y);
-        __syncthreads();
-        load_cv(now);
-        // A part of the softmax in the shadow of each MFMA; LDS reads run LOOK entries
-        // ahead of theirs.  sched_barrier keeps the steps apart: left to itself the
-        // compiler lines the MFMAs up behind the exponentials.
-        constexpr int LOOK = 3;
-        const uint16_t* const Kn = tile0 + next * Tl::kTile + li * K_RS + 8 * g;
-        u32x4 ka[KS], va[2 * DB];
+      load_cv(now);
+      // A part of the softmax in the shadow of each MFMA; LDS reads run LOOK entries
+      // ahead of theirs.  sched_barrier keeps the steps apart: left to itself the
+      // compiler lines the MFMAs up behind the exponentials.
+      constexpr int LOOK = 3;
+      const uint16_t* const Kn = tile0 + next * Tl::kTile + li * K_RS + 8 * g;
+      u32x4 ka[KS], va[2 * DB];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s2[r] = 0.f;
+      for (int r = 0; r < 16; ++r) s2[r] = 0.f;
 #pragma unroll
-        for (int k = 0; k < LOOK; ++k) ka[k] = *reinterpret_cast<const u32x4*>(Kn + 16 * k);
+      for (int k = 0; k < LOOK; ++k) ka[k] = *reinterpret_cast<const u32x4*>(Kn + 16 * k);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        s2 = Mfma<QT>::mma(ka[k], qf[k], s2);
+        if (k + LOOK < KS) ka[k + LOOK] = *reinterpret_cast<const u32x4*>(Kn + 16 * (k + LOOK));
+        else va[k + LOOK - KS] = read_v(now, k + LOOK - KS);
+#pragma unroll
+        for (int j = 8 * k / KS; j < 8 * (k + 1) / KS; ++j) piece(s, j);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          s2 = Mfma<QT>::mma(ka[k], qf[k], s2);
-          if (k + LOOK < KS) ka[k + LOOK] = *reinterpret_cast<const u32x4*>(Kn + 16 * (k + LOOK));
-          else va[k + LOOK - KS] = read_v(now, k + LOOK - KS);
-#pragma unroll
-          for (int j = 8 * k / KS; j < 8 * (k + 1) / KS; ++j) piece(s, j);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        float mx = 0.f;
-#pragma unroll
-        for (int e = 0; e < 2 * DB; ++e) {
-          pv(va[e], e);
-          if (e + LOOK < 2 * DB) va[e + LOOK] = read_v(now, e + LOOK);
-          if (e == DB / 2 - 1) {
-            scale_s(s2, next);
-            mask(s2, t + KG);
-          }
-          if (e == DB) mx = largest(s2);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        raise(mx);
-        store_k(X, now);
-        store_v(X, t + KG, next);
-      };
-      for (int i = 0; i < rounds; i += 2) {
-        round(i, sa, sb, Rb, Ra);
-        if (i + 1 < rounds) round(i + 1, sb, sa, Ra, Rb);  // uniform
       }
+      float mx = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2 * DB; ++e) {
+        pv(va[e], e);
+        if (e + LOOK < 2 * DB) va[e + LOOK] = read_v(now, e + LOOK);
+        if (e == DB / 2 - 1) {
+          scale_s(s2, next);
+          mask(s2, i + 1);
+        }
+        if (e == DB) mx = largest(s2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      raise(mx);
+      store_k(X, now);
+      store_v(X, i + 1, next);
+    };
+    for (int i = 0; i < n_tiles; i += 2) {
+      round(i, sa, sb, Rb, Ra);
+      if (i + 1 < n_tiles) round(i + 1, sb, sa, Ra, Rb);  // uniform
     }
   }
 
@@ -577,8 +568,8 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
     __syncthreads();  // every wave is done with its tiles
     float* so = reinterpret_cast<float*>(smem);       // [waves][32][OS]
     float* sml = so + kSharedWaves * 32 * OS;         // [waves][32][2]
-    const int nvalid = min(32 * RB, R - row0);
-    if (32 * rb + li < nvalid) {
+    const int nvalid = min(32, R - row0);
+    if (li < nvalid) {
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -594,15 +585,14 @@ __device__ __forceinline__ void shared_segment(const SharedParams& p, uint8_t* s
     for (int idx = threadIdx.x; idx < nvalid * (D / 4); idx += kSharedWaves * 64) {
       const int r = idx / (D / 4);
       const int d = 4 * (idx - r * (D / 4));
-      const int at0 = (r >> 5) * 32 + (r & 31);  // key group 0's; the next ones' lie RB waves on
       float M = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < KG; ++k) M = fmaxf(M, sml[(k * RB * 32 + at0) * 2]);
+      for (int k = 0; k < KG; ++k) M = fmaxf(M, sml[(k * 32 + r) * 2]);
       f32x4 A = {0.f, 0.f, 0.f, 0.f};
       float L = 0.f;
 #pragma unroll
       for (int k = 0; k < KG; ++k) {
-        const int at = k * RB * 32 + at0;
+        const int at = k * 32 + r;
         const float m = sml[at * 2];
         const float f = m == -INFINITY ? 0.f : fast_exp2(m - M);  // a NaN in l or acc stays one
         A += *reinterpret_cast<const f32x4*>(&so[at * OS + d]) * f;

@@ -326,7 +326,9 @@ def paged_decode_attention_shared(
     128) run as ordinary decode, which reads the prefix once per sequence, and per
     token of a multi-token query, and so do batches without ``scales`` in which no
     two sequences share a key; ``config`` does not apply to the former.  K and V
-    rows are 16-byte aligned, as for every decode.  Returns ``q``'s shape and dtype.
+    rows are 16-byte aligned, as for every decode.  On fp16 caches the softmax's
+    numerators are rounded to fp16 (in bf16 and on 8-bit caches to two bf16 parts).
+    Returns ``q``'s shape and dtype.
     """
     _check_inputs(q, cache, cu_groups, prefix_lens, scales)
     _require_rocm(q, cache, "paged_decode_attention_shared")

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from flashattntile_amd import PagedKVCache
+from flashattntile_amd import PagedKVCache, _hip
 from flashattntile_amd.kernels.shared import paged_decode_shared_launch, shared_splits
 
 
@@ -70,3 +70,17 @@ def test_partials_stay_below_a_ceiling(batch, tokens, big):
             for small in (1, big):
                 cfg, bytes_ = _partials(batch, tokens, big, small, heads, kv_heads, prefix)
                 assert bytes_ <= 2 ** 29 or cfg["prefix_split"] == cfg["split"] == 1
+
+
+@pytest.mark.parametrize("shape", [(3, 4, 64), (3, 5, 4, 64), (1, 2, 64)])
+@pytest.mark.parametrize("splits", [(1, 1), (7, 3), (64, 64)])
+def test_the_launch_allocates_what_the_library_says(monkeypatch, shape, splits):
+    given = []
+    monkeypatch.setattr(_hip, "current_stream_handle", lambda device: 0)
+    monkeypatch.setattr(_hip, "shared_with_args", lambda a, workspace, stream: given.append(workspace.numel()))
+    batch, k = shape[0], torch.zeros(12, 8, 2, 64, dtype=torch.float16)
+    cache = PagedKVCache(k, k.clone(), torch.zeros(batch, 4, dtype=torch.int32), _ints([20] * batch), 8)
+    paged_decode_shared_launch(torch.zeros(shape, dtype=torch.float16), cache, _ints([0, batch]), _ints([16]), 0.125, 16,
+                               9, config={"prefix_split": splits[0], "split": splits[1]})
+    rows = batch * (shape[1] if len(shape) == 4 else 1)
+    assert given == [_hip.lib().fat_paged_decode_shared_workspace_bytes(rows, shape[-2], 64, sum(splits))]
