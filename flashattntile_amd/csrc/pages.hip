@@ -170,7 +170,8 @@ struct ForkParams {
 };
 
 // 240 forks of pages of 384 KiB (with their 8-bit copy) take 39 us: 92 MB written,
-// 2.4 TB/s, as a copy's writes.
+// 2.4 TB/s.  A fill of as much takes 15 us and torch's copy of 16 such pages to 240
+// places 34, so its writes alone don't bound it.
 // blockIdx.y: the fork; blockIdx.z: a plane of its last page, or (the last) its
 // table row; blockIdx.x: steps.  Every workgroup of a fork reads only its
 // parent's row, which no fork of the call writes, and decides alike.
