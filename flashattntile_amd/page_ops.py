@@ -24,8 +24,8 @@ strided int32 vectors on the cache's device.  On a ROCm cache the work is HIP
 kernels on the current stream (``csrc/pages.hip``) and the checks cost one
 launch that the host polls; ``validate=False`` leaves them out (capture, serving
 loops): pairs and rows that are out of range are then skipped on the device.
-CPU caches take torch, always checked.  Bad arguments raise ``AssertionError``, as the cache's
-other checks do, before anything is changed.
+CPU caches take torch, always checked.  Bad arguments raise ``AssertionError``,
+as the cache's other checks do, before anything is changed.
 """
 
 from __future__ import annotations
